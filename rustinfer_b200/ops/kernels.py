@@ -2025,3 +2025,181 @@ def sample(logits: torch.Tensor, scratch: torch.Tensor, temperature: torch.Tenso
 def sample_scratch_elems(rows: int, vocab: int) -> int:
     """int64 words of scratch for `rows` rows: room for the rows that are sorted whole, and a flag a row."""
     return rows * (1 << max(1, (vocab - 1).bit_length())) + rows
+
+
+# ------------------------------------------------------------------------------------------------ beam search
+BEAMS_MAX, BEAM_PICKS_MAX = 64, 128
+
+
+def _on_current_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Kernels are launched on the current device's stream: tensors of another one are refused, not reached over its back."""
+    current = L._current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != current:
+            raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{current}")
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, out_scores: torch.Tensor, out_rows: torch.Tensor,
+                out_tokens: torch.Tensor) -> None:
+    """The best continuations of every group of `beams` rows: score(r, t) = scores[r] + log softmax(logits[r])[t].
+
+    logits fp32 [groups * beams, vocab] (unit column stride, any row stride), scores fp32 [groups * beams].  The outputs
+    [groups, picks] get, best first, the scores (fp32), the rows they continue (int32, counted over all groups) and the
+    tokens (int32).  Equal scores go by ascending (row, token); scores are compared in 64 bits.  A row whose score is -inf
+    has no continuation but of score -inf, and neither has a token whose logit is -inf or not a number.  In a row that
+    holds +inf, those tokens share the weight.  Up to 64 beams and 128 picks."""
+    require_cuda(logits, scores, out_scores, out_rows, out_tokens)
+    _on_current_device("beam_select", logits, scores, out_scores, out_rows, out_tokens)
+    if logits.dtype != torch.float32 or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise KernelError("beam_select: logits are fp32 [rows, vocab] with unit column stride")
+    R, V = logits.shape
+    if not 1 <= beams <= BEAMS_MAX or R % beams:
+        raise KernelError(f"beam_select: {R} rows are no groups of {beams} (1 to {BEAMS_MAX})")
+    if scores.dtype != torch.float32 or scores.numel() != R:
+        raise KernelError(f"beam_select: scores are fp32 [{R}]")
+    groups = R // beams
+    picks = out_scores.shape[-1]
+    for t, n, dt in ((out_scores, "out_scores", torch.float32), (out_rows, "out_rows", torch.int32), (out_tokens, "out_tokens", torch.int32)):
+        if t.dtype != dt or t.shape != (groups, picks):
+            raise KernelError(f"beam_select: {n} is {dt} [{groups}, {picks}], got {t.dtype} {tuple(t.shape)}")
+        _contig(t, n)
+    _contig(scores, "scores")
+    if not 1 <= picks <= min(BEAM_PICKS_MAX, beams * V):
+        raise KernelError(f"beam_select: {picks} picks of {beams} x {V} continuations (1 to {BEAM_PICKS_MAX})")
+    if R == 0:
+        return
+    if R > 65535 or V > 1 << 30:
+        raise KernelError(f"beam_select: {R} rows of {V} tokens (up to 65,535 rows and 2^30 tokens)")
+    lib, sms = L.beams(), L.num_sms(logits.device)
+    # a sum (16 bytes) and the best (8 each) of every slice of every row
+    scratch = torch.empty(R * lib.ri_beam_select_slices(R, V, sms) * (2 + picks), dtype=torch.int64, device=logits.device)
+    check(lib.ri_beam_select(_p(logits), logits.stride(0), V, _p(scores), groups, beams, picks, sms, _p(scratch), _p(out_scores), _p(out_rows),
+                             _p(out_tokens), stream_ptr()), "beam_select", 2)
+
+
+def _row_sizes(what: str, store: torch.Tensor, tokens: Optional[torch.Tensor], n: int) -> Tuple[int, int, int, int, int]:
+    """(layers, rows, bytes a row, bytes a segment, bytes a token) of a cache's storage."""
+    if store.dim() < 2:
+        raise KernelError(f"{what}: the storage is [layers, rows, ...], got {tuple(store.shape)}")
+    _contig(store, "store")
+    layers, total = store.shape[:2]
+    row = store[0, 0].numel() * store.element_size() if store.numel() else 0
+    if tokens is None:
+        return layers, total, row, row, row
+    _i32(tokens, "tokens")
+    if store.dim() != 6 or store.shape[2] != 2 or tokens.numel() != n:
+        raise KernelError(f"{what}: tokens are int32 [{n}], for pages [layers, pages, 2, kv heads, page, head_dim]")
+    _contig(tokens, "tokens")
+    token = store.shape[5] * store.element_size()
+    return layers, total, row, store.shape[4] * token, token
+
+
+def reorder_rows(store: torch.Tensor, rows: torch.Tensor, parents: torch.Tensor, beams: int, tokens: Optional[torch.Tensor] = None) -> None:
+    """store[:, rows[r]] = store[:, rows[parents[r]]] for every r, in place, as if all were read before any is written.
+
+    store [layers, rows in all, ...] contiguous, of any type: state slots, or pages.  rows and parents int32 [groups * beams];
+    a parent is a place in `rows` (counted over all groups, as `beam_select` gives it) of the same group, any mapping at all.
+    With `tokens` (int32 [groups * beams]) the storage is pages [layers, pages, 2, kv heads, page, head_dim], and only the
+    first tokens[r] tokens of a page are taken over.  A parent outside the group and a row outside the storage leave the row
+    as it is.  No row may be listed twice."""
+    require_cuda(store, rows, parents, tokens)
+    _on_current_device("reorder_rows", store, rows, parents, tokens)
+    _i32(rows, "rows"); _i32(parents, "parents"); _contig(rows, "rows"); _contig(parents, "parents")
+    n = rows.numel()
+    if not 1 <= beams <= BEAMS_MAX or n % beams or parents.numel() != n:
+        raise KernelError(f"reorder_rows: {n} rows and {parents.numel()} parents are no groups of {beams} (1 to {BEAMS_MAX})")
+    layers, total, row, seg, token = _row_sizes("reorder_rows", store, tokens, n)
+    if n == 0 or layers == 0 or row == 0 or total == 0:
+        return
+    if layers > 65535 or n // beams > 65535 or row >= 1 << 31:
+        raise KernelError(f"reorder_rows: {layers} layers, {n // beams} groups, rows of {row} bytes (below 65,536, 65,536 and 2^31)")
+    check(L.beams().ri_reorder_rows(_p(store), layers, total, row, seg, token, _p(rows), _p(parents), n // beams, beams, _p(tokens), stream_ptr()),
+          "reorder_rows")
+
+
+def copy_pages(store: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, tokens: Optional[torch.Tensor] = None) -> None:
+    """store[:, dst[i]] = store[:, src[i]] for every i, in every layer: a fork's last page, or pages on their way to lower numbers.
+
+    store [layers, pages, ...] contiguous, of any type; src and dst int32 [n].  With `tokens` (int32 [n]) the storage is
+    [layers, pages, 2, kv heads, page, head_dim] and only the first tokens[i] tokens are copied.  A page outside the storage
+    and a page copied to itself are left out.  A page may be the source of many copies; no page may be the destination of
+    two, and no destination may be a source (the copies run side by side)."""
+    require_cuda(store, src, dst, tokens)
+    _on_current_device("copy_pages", store, src, dst, tokens)
+    _i32(src, "src"); _i32(dst, "dst"); _contig(src, "src"); _contig(dst, "dst")
+    n = src.numel()
+    if dst.numel() != n:
+        raise KernelError(f"copy_pages: {n} sources, {dst.numel()} destinations")
+    layers, total, row, seg, token = _row_sizes("copy_pages", store, tokens, n)
+    if n == 0 or layers == 0 or row == 0 or total == 0:
+        return
+    if layers > 65535 or row >= 1 << 31:
+        raise KernelError(f"copy_pages: {layers} layers, pages of {row} bytes (below 65,536 and 2^31)")
+    check(L.beams().ri_copy_pages(_p(store), layers, total, row, seg, token, _p(src), _p(dst), n, _p(tokens), stream_ptr()), "copy_pages")
+
+
+def attention_beams_supports(num_heads: int, num_kv_heads: int, head_dim: int) -> bool:
+    return num_kv_heads > 0 and num_heads % num_kv_heads == 0 and head_dim % 16 == 0 and 16 <= head_dim <= L.MMA_MAX_HEAD_DIM
+
+
+@functools.lru_cache(maxsize=4096)
+def attention_beams_splits(rows: int, beams: int, num_heads: int, num_kv_heads: int, head_dim: int, most_shared: int, most_own: int,
+                           num_sms: int) -> Tuple[int, int]:
+    """Ranges that the shared keys of a group, and the keys of a row's own, are cut into: about a wave of CTAs for the former."""
+    lib = L.attention_beams(head_dim)
+    group = num_heads // num_kv_heads
+    row_tiles = int(lib.ri_attention_beams_row_tiles(beams * group))
+    slots = int(lib.ri_attention_beams_ctas_per_sm(row_tiles)) * num_sms
+    ctas = rows // beams * num_kv_heads * -(-beams * group // (16 * row_tiles))
+    shared = max(1, min(slots // max(1, ctas), -(-most_shared // 128), 16))
+    return shared, max(1, min(-(-most_own // 256), 8))
+
+
+def attention_decode_beams(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,
+                           shared_len: torch.Tensor, beams: int, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
+                           window: Optional[int], most_shared: int, most_own: int, part_o: Optional[torch.Tensor] = None,
+                           part_lse: Optional[torch.Tensor] = None) -> None:
+    """`attention_decode_bf16` for rows that are beams: row r, one token, sees the kv_len[r] keys (the last `window` of them) that
+    its row of the block table gives, and the first shared_len[g] are the same for all rows of its group g = r // beams, whatever
+    pages they lie in.  These are read once for the group, by its first row's table.
+
+    q, out bf16 [rows, heads * head_dim] (unit column stride), cache bf16 [pages, 2, kv heads, page, head_dim], block_table int32
+    [rows, pages a row], kv_len int32 [rows], shared_len int32 [rows / beams].  A row without keys gets zeros.  A group one of
+    whose rows has fewer keys than shared_len, or whose rows' windows start at different keys, is read row by row.
+    most_shared and most_own: about how many keys the longest shared part and the longest rest have (they choose how the work is
+    cut, not what is computed).  part_o, part_lse: fp32 scratch (`decode_scratch_floats` with the sum of
+    `attention_beams_splits`); without them it is allocated."""
+    require_cuda(q, out, cache, block_table, kv_len, shared_len, part_o, part_lse)
+    _on_current_device("attention_decode_beams", q, out, cache, block_table, kv_len, shared_len, part_o, part_lse)
+    for t, n in ((block_table, "block_table"), (kv_len, "kv_len"), (shared_len, "shared_len")):
+        _i32(t, n)
+    if not attention_beams_supports(num_heads, num_kv_heads, head_dim):
+        raise KernelError(f"attention_decode_beams: {num_heads} heads over {num_kv_heads} of {head_dim} (a multiple of 16 up to {L.MMA_MAX_HEAD_DIM})")
+    R = q.shape[0]
+    if not 1 <= beams <= BEAMS_MAX or R % beams:
+        raise KernelError(f"attention_decode_beams: {R} rows are no groups of {beams} (1 to {BEAMS_MAX})")
+    for t, n in ((q, "q"), (out, "out")):
+        if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape != (R, num_heads * head_dim) or t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+            raise KernelError(f"attention_decode_beams: {n} is bf16 [{R}, {num_heads * head_dim}] with unit column stride")
+    if q.stride(0) % 8 or q.data_ptr() % 16 or cache.data_ptr() % 16:
+        raise KernelError("attention_decode_beams: rows of q and the cache start on 16-byte boundaries")
+    if cache.dtype != torch.bfloat16 or cache.dim() != 5 or cache.shape[1] != 2 or cache.shape[2] != num_kv_heads or cache.shape[4] != head_dim:
+        raise KernelError("attention_decode_beams: cache is bf16 [pages, 2, kv heads, page, head_dim]")
+    _contig(cache, "cache"); _contig(kv_len, "kv_len"); _contig(shared_len, "shared_len")
+    if block_table.dim() != 2 or block_table.shape[0] < R or block_table.stride(1) != 1 or kv_len.numel() < R or shared_len.numel() < R // beams:
+        raise KernelError(f"attention_decode_beams: a block table and a length for {R} rows, a shared length for {R // beams} groups")
+    if window is not None and window < 1:
+        raise KernelError(f"attention_decode_beams: a window of {window} keys")
+    if R == 0:
+        return
+    splits = attention_beams_splits(R, beams, num_heads, num_kv_heads, head_dim, max(0, int(most_shared)), max(1, int(most_own)), L.num_sms(q.device))
+    need_o, need_l = decode_scratch_floats(R, num_heads, head_dim, sum(splits))
+    if part_o is None or part_lse is None:
+        scratch = torch.empty(need_o + need_l, dtype=torch.float32, device=q.device)
+        part_o, part_lse = scratch[:need_o], scratch[need_o:]
+    if part_o.dtype != torch.float32 or part_lse.dtype != torch.float32 or part_o.numel() < need_o or part_lse.numel() < need_l:
+        raise KernelError(f"attention_decode_beams: scratch must hold {need_o} and {need_l} fp32")
+    check(L.attention_beams(head_dim).ri_attention_beams(
+        _p(q), q.stride(0), _p(out), out.stride(0), _p(cache), _p(block_table), block_table.stride(0), block_table.shape[1], _p(kv_len),
+        _p(shared_len), R // beams, beams, num_heads, num_kv_heads, cache.shape[3], float(scale), int(window or 0), splits[0], splits[1], _p(part_o),
+        _p(part_lse), stream_ptr()), "attention_decode_beams", 2)

@@ -98,6 +98,13 @@ _SIGNATURES = {
     "ri_part_norm_gate": [_P, _P, _I, _P, _I, _P, _I, _P, _F, _I, _P, _I, _I, _I, _I, _P],
     "ri_embed_pairs": [_P, _P, _P, _I, _P, _P, _P, _I, _F, _P, _I, _L, _L, _L, _P, _I, _I, _I, _P],
     "ri_token_gate": [_P, _I, _P, _P, _I, _I, _I, _I, _P, _I, _I, _I, _P],
+    "ri_beam_select_slices": [_I, _I, _I],
+    "ri_beam_select": [_P, _L, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P],
+    "ri_reorder_rows": [_P, _I, _L, _L, _L, _L, _P, _P, _I, _I, _P, _P],
+    "ri_copy_pages": [_P, _I, _L, _L, _L, _L, _P, _P, _I, _P, _P],
+    "ri_attention_beams": [_P, _I, _P, _I, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _I, _P, _P, _P],
+    "ri_attention_beams_row_tiles": [_I],
+    "ri_attention_beams_ctas_per_sm": [_I],
     "ri_gated_decay": [_P, _P, _I, _F, _I, _I, _P],
     "ri_delta_prepare": [_P, _I, _P, _I, _P, _P, _P, _I, _I, _F, _F, _P, _P, _I, _I, _I, _P],
 }
@@ -235,14 +242,28 @@ def attention_tc(head_dim: int) -> ctypes.CDLL:
     return _load(f"ri_attention_tc_hd{head_dim}", ["attention_tc.cu"], [f"RI_HEAD_DIM={head_dim}"])
 
 
+def beams() -> ctypes.CDLL:
+    """Beam search's choice, and the rows and pages that move with it."""
+    return _load("ri_beams", ["beam_select.cu", "beam_rows.cu"])
+
+
+def attention_beams(head_dim: int) -> ctypes.CDLL:
+    """The decode attention of beams that share their prompt's keys."""
+    if head_dim % 16 != 0 or not 16 <= head_dim <= MMA_MAX_HEAD_DIM:
+        raise KernelError(f"the attention of beams takes head sizes that are multiples of 16 up to {MMA_MAX_HEAD_DIM}, got {head_dim}")
+    return _load(f"ri_attention_beams_hd{head_dim}", ["attention_beams.cu"], [f"RI_HEAD_DIM={head_dim}"])
+
+
 def build_all(head_dims) -> None:
     """Compile every library for the given head sizes (the ahead-of-time build check)."""
     core()
     gemm_tc()
+    beams()
     for hd in head_dims:
         attention_plain(hd)
         if hd <= MMA_MAX_HEAD_DIM:
             attention_mma(hd)
+            attention_beams(hd)
         if hd in (64, 128):
             attention_tc(hd)
 
