@@ -293,7 +293,7 @@ beams_kernel(Args a, int groups, int chunks, int own_chunks) {
 }
 
 // out[r, h, :] = sum over ranges of 2^(lse - max) part / sum of 2^(lse - max); a row without keys: zeros
-__global__ void beams_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse, bf16* __restrict__ out, int out_stride, int Hq,
+__global__ void beams_join_kernel(const float* part_o, const float* part_lse, bf16* out, int out_stride, int Hq,
                                   int splits) {
     pdl_wait();
     const int r = blockIdx.x, h = blockIdx.y;

@@ -31,7 +31,7 @@ __device__ __forceinline__ int used_of(const Extent& x, int i) {
 
 template <typename V, int U>
 __global__ void __launch_bounds__(RT)
-reorder_rows_kernel(V* __restrict__ store, long long total, int row_vectors, const int* __restrict__ rows, const int* __restrict__ parents,
+reorder_rows_kernel(V* store, long long total, int row_vectors, const int* rows, const int* parents,
                     int beams, Extent extent) {
     __shared__ int m_src[2 * MAX_BEAMS], m_dst[2 * MAX_BEAMS], m_used[2 * MAX_BEAMS];
     __shared__ int n_moves, cyclic;
@@ -144,7 +144,7 @@ reorder_rows_kernel(V* __restrict__ store, long long total, int row_vectors, con
 
 template <typename V, int U>
 __global__ void __launch_bounds__(RT)
-copy_pages_kernel(V* __restrict__ store, long long total, int row_vectors, int chunks, const int* __restrict__ src, const int* __restrict__ dst,
+copy_pages_kernel(V* store, long long total, int row_vectors, int chunks, const int* src, const int* dst,
                   Extent extent) {
     pdl_wait();
     const int i = blockIdx.x / chunks, chunk = blockIdx.x - i * chunks;

@@ -6,24 +6,31 @@
 // (crates/infer-worker/src/application/sampler_stack.rs:242-351) and has no counterpart.
 //
 // Within a row a score falls with its logit, so the row's own best `picks` logits are all that can be chosen, and the
-// logits are read once: a CTA holds a slice of a row in registers, sums exp(x - slice maximum), and finds the slice's
-// best.  These two are all that leaves the CTA; a second kernel, a CTA a group, puts the slices' sums together in 64
+// logits are read once: a CTA walks a slice of a row, keeps the sum of its weights and what may be among the slice's best.
+// These two are all that leaves the CTA; a second kernel, a CTA a group, puts the slices' sums together in 64
 // bits, scores what the slices sent in 64 bits and orders it.
 //
 // The best `picks` of a slice without a sort: let t be a value that at least `picks` threads' own maxima reach; then at
 // least `picks` elements reach it and nothing below it is among the best.  t is found by bisection on the maxima, a
-// barrier with a count a step, and stops as soon as no more than twice `picks` threads are left.  The few elements that
-// reach t are gathered and a warp counts the ones ahead of each: its rank is its place.  A slice in which more than the
-// gathering's room reach t (thousands of equal logits, words that are forbidden) finds the last element that belongs
-// to the best exactly, by bisection over values and then over indices.
+// barrier with a count a step, and stops as soon as no more than one and a half times `picks` threads are left.  The few elements
+// that reach t leave the CTA as they come; in a slice of several chunks they are found by each thread's maximum of every chunk,
+// and those few chunks are read once more (from L2).  Where more than twice `picks` do, a warp counts the ones ahead of
+// each, which is its rank, and the best `picks` leave.  Where more than the gathering's room reach t (thousands of equal logits,
+// words that are forbidden), the last element that belongs is found exactly, by bisection over values and then over indices.
+// The second kernel does the same with 64-bit scores.
 //
 // Scores and the sums over slices are 64-bit: the rows of a group compete through the sums, and a choice hangs on
 // differences however small.  Weights are 32-bit exponentials, summed in 32 bits over a warp's elements and in 64 from there.
 #include "common.cuh"
 
 namespace {
-constexpr int ST = 512;                                    // threads of a slice
-constexpr int MT = 512;                                    // threads of a group
+constexpr int ST = 256;                                    // threads of a slice
+constexpr int NV = 4;                                      // 16-byte loads of a thread a chunk
+constexpr int CTAS = 3;                                    // CTAs an SM, which walk over slices
+constexpr int STAGES = 3;                                  // chunks of a slice in flight
+constexpr int MAX_CHUNKS = 8;                              // chunks of a slice
+constexpr int LISTS = 1024;                                // slices of a group whose sums are kept in shared memory
+constexpr int MT = 512;                                   // threads of a group
 constexpr int CAP = 1024;                                  // room of the gathering
 constexpr int MAX_PICKS = 128, MAX_BEAMS = 64;
 
@@ -37,11 +44,24 @@ __device__ __forceinline__ float from_ordered(unsigned k) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
-struct SliceStat {                                         // sum of exp(x - m) over a slice
+constexpr float L = 1.4426950408889634f;                   // log2 e in 32 bits
+// A slice's sum of weights, its largest logit, and how many of its elements left the CTA.  The weights are 2^(x L - ref) with
+// ref = ceil(m L), or exp(x - m) where `by_difference`
+struct SliceStat {
     double sum;
     float m;
-    int pad;
+    int n;
 };
+__device__ __forceinline__ bool by_difference(float m) { return !(fabsf(m) <= 65536.f); }      // beyond, x L - ref is not near enough
+__device__ __forceinline__ float whole_ref(float m) { return ceilf(m * L); }
+__device__ __forceinline__ float two_to(float whole) {     // 2^whole for a whole number up to 0, exactly; 0 below the normal numbers
+    return whole < -126.f ? 0.f : __int_as_float((127 + (int)whole) << 23);
+}
+__device__ __forceinline__ float ex2(float x) {            // 2 ulp
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // count of a block's elements (each thread brings its own)
 __device__ __forceinline__ int block_count(int mine, int* cell) {
@@ -63,7 +83,7 @@ __device__ __forceinline__ unsigned reach(unsigned mine, unsigned floor, unsigne
         const int n = __syncthreads_count(mine >= mid);
         if (n >= picks) {
             lo = mid;
-            if (n <= 2 * picks) break;
+            if (2 * n <= 3 * picks) break;
         } else {
             hi = mid - 1;
         }
@@ -71,139 +91,256 @@ __device__ __forceinline__ unsigned reach(unsigned mine, unsigned floor, unsigne
     return lo;
 }
 
-template <int NV>
-__global__ void __launch_bounds__(ST, 2)
-beam_slices_kernel(const float* __restrict__ logits, long long ld, int vocab, const float* __restrict__ scores, int picks,
-                   int vectors_a_slice, unsigned long long* __restrict__ best, SliceStat* __restrict__ stat) {
+__device__ __forceinline__ void copy_async16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_async4(void* to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+
+__global__ void __launch_bounds__(ST, CTAS)
+beam_slices_kernel(const float* logits, long long ld, int vocab, const float* scores, int picks, int items, int slices,
+                   int vectors_a_slice, unsigned long long* best, SliceStat* stat) {
+    extern __shared__ float4 ring[];                       // [STAGES][NV][W][33]: a warp reads what it has fetched itself, so no barrier
     __shared__ unsigned long long list[CAP];
-    __shared__ float wmax[ST / 32];
+    __shared__ unsigned red_hi[ST / 32], red_lo[ST / 32];
     __shared__ float wsum[ST / 32];
+    __shared__ float chunk_top[MAX_CHUNKS][ST];
+    __shared__ unsigned short again[MAX_CHUNKS * ST];
     __shared__ int cell, listed;
-    const int slice = blockIdx.x, slices = gridDim.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    unsigned long long* const mine_best = best + ((size_t)r * slices + slice) * picks;
-    SliceStat* const mine_stat = stat + (size_t)r * slices + slice;
-    if (tid == 0) listed = 0;
+    constexpr int W = ST / 32, CHUNK = NV * ST;
+    constexpr unsigned MINUS_INF = 0x007fffffu;            // ordered(-inf)
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
     pdl_trigger();
-    const float* const row = logits + (size_t)r * ld;
-    // An element's thread goes by its index alone, whatever the row's alignment: equal rows get equal sums, and their
-    // continuations are equals that go by index.  A row off a 16-byte boundary is read in single elements.
-    const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
-    const int v0 = slice * vectors_a_slice, v1 = min(v0 + vectors_a_slice, (vocab + 3) >> 2);
-    const int e_lo = 4 * v0, e_hi = min(vocab, 4 * v1);    // the slice's elements
-    const float s_row = scores[r];
-    if (!(s_row > -INFINITY)) {                            // a row without a future: every score -inf, by index
-        for (int i = tid; i < picks; i += ST)
-            mine_best[i] = e_lo + i < e_hi ? (0x007fffffull << 32) | (unsigned)(0xffffffffu - (unsigned)(e_lo + i)) : 0ull;
-        if (tid == 0) *mine_stat = SliceStat{0.0, -INFINITY, 0};
-        return;
-    }
-    float x[4 * NV];
+    struct Slice {                                         // of row r, vectors v0 .. v1 - 1, elements up to e_hi
+        const float* row;
+        int v0, v1, e_hi, shift;                           // the row starts `shift` elements behind a 16-byte boundary
+        bool dead;
+    } now, then;
+    auto open = [&](Slice& s, int item) {
+        const int r = item / slices;
+        s.row = logits + (size_t)r * ld;
+        s.v0 = (item - r * slices) * vectors_a_slice;
+        s.v1 = min(s.v0 + vectors_a_slice, (vocab + 3) >> 2);
+        s.e_hi = min(vocab, 4 * s.v1);
+        s.shift = (int)((reinterpret_cast<uintptr_t>(s.row) >> 2) & 3);
+        s.dead = !(scores[r] > -INFINITY);                 // without a future: not read
+    };
+    // A vector of the ring holds 16 aligned bytes: where the row starts `shift` elements behind a boundary, a thread's four elements lie in
+    // its own and in the next lane's, and the warp fetches a 33rd.
+    auto fetch = [&](const Slice& s, int v, int stage) {
+        if (v < s.v1 && !s.dead) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int v = v0 + i * ST + tid, e = 4 * v;
-        if (aligned && v < v1 && e + 4 <= vocab) {
-            const float4 f = __ldcs(reinterpret_cast<const float4*>(row + e));
-            x[4 * i] = f.x; x[4 * i + 1] = f.y; x[4 * i + 2] = f.z; x[4 * i + 3] = f.w;
-        } else {
+            for (int i = 0; i < NV; ++i) {
+                float4* const to = ring + ((stage * NV + i) * W + warp) * 33;
+                const int first = v + i * ST + warp * 32;
+                for (int j = lane; j < 32 + (s.shift != 0); j += 32) {
+                    const int e = 4 * (first + j) - s.shift;
+                    if (e >= 0 && e + 4 <= s.e_hi) {
+                        copy_async16(to + j, s.row + e);
+                    } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[4 * i + k] = v < v1 && e + k < vocab ? row[e + k] : -INFINITY;
+                        for (int k = 0; k < 4; ++k)
+                            if (e + k >= 0 && e + k < s.e_hi) copy_async4(reinterpret_cast<float*>(to + j) + k, s.row + e + k);
+                            else reinterpret_cast<float*>(to + j)[k] = -INFINITY;
+                    }
+                }
+            }
         }
-    }
-    float top = -INFINITY;
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+    };
+    auto prime = [&](const Slice& s) {
 #pragma unroll
-    for (int i = 0; i < 4 * NV; ++i) {
-        x[i] = fmaxf(x[i], -INFINITY);                     // what is no number has no chance
-        top = fmaxf(top, x[i]);
+        for (int c = 0; c < STAGES - 1; ++c) fetch(s, s.v0 + c * CHUNK, c);
+    };
+    if ((int)blockIdx.x < items) {
+        open(then, blockIdx.x);
+        prime(then);
     }
-    const unsigned own_top = key_of(top);
-    top = from_ordered(__reduce_max_sync(0xffffffffu, own_top));
-    if (lane == 0) wmax[warp] = top;
-    __syncthreads();
-    float m = wmax[lane & (ST / 32 - 1)];
-    m = from_ordered(__reduce_max_sync(0xffffffffu, ordered(m)));
-    float sum = 0.f;
-    if (m == INFINITY) {                                   // the weight lies on the infinite ones alone
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    now = then;
+    const float* const row = now.row;
+    const int v0 = now.v0, v1 = now.v1, e_lo = 4 * v0, e_hi = now.e_hi, count = max(0, e_hi - e_lo);
+    unsigned long long* const mine_best = best + (size_t)item * (2 * picks);
+    SliceStat* const mine_stat = stat + item;
+    __syncthreads();                                       // the slice before is done with what the block shares
+    if (tid == 0) cell = listed = 0;
+    auto next = [&]() {
+        if (item + (int)gridDim.x < items) {
+            open(then, item + gridDim.x);
+            prime(then);                                   // on its way while this slice's end is made
+        }
+    };
+    if (now.dead) {                                        // every score -inf, by index
+        for (int i = tid; i < min(picks, count); i += ST) mine_best[i] = ((unsigned long long)MINUS_INF << 32) | (unsigned)(0xffffffffu - (unsigned)(e_lo + i));
+        if (tid == 0) *mine_stat = SliceStat{0.0, -INFINITY, min(picks, count)};
+        next();
+        continue;
+    }
+    // A thread's sum of 2^(x L - ref), L = log2 e in 32 bits, ref a whole number that is at least the thread's largest x L: one fused
+    // multiply-add an element, whose own rounding is all that is lost, and moving on to another ref is exact.
+    float sum = 0.f, ref = -1e30f, top = -INFINITY;        // (top: what is no number does not count)
+    auto add_up = [&](const float (&x)[4 * NV], float high) {
+        const float to = fmaxf(ref, ceilf(high * L));
+        float part[4] = {sum * ex2(ref - to), 0.f, 0.f, 0.f};
+        ref = to;
 #pragma unroll
-        for (int i = 0; i < 4 * NV; ++i) sum += x[i] == INFINITY ? 1.f : 0.f;
-    } else if (m > -INFINITY) {
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 4 * NV; ++i) part[i & 3] += ex2(fmaf(x[i], L, -to));
+        sum = (part[0] + part[1]) + (part[2] + part[3]);
+    };
+    auto highest = [&](const float (&x)[4 * NV]) {
+        float h[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 4 * NV; ++i) h[i & 3] = fmaxf(h[i & 3], x[i]);
+        return fmaxf(fmaxf(h[0], h[1]), fmaxf(h[2], h[3]));
+    };
+    unsigned t = 0;                                        // a value that the slice's best all reach (0: all do)
+    float tf = -INFINITY;
+    auto gather = [&](const float (&x)[4 * NV], int v) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
+            if (!(fmaxf(fmaxf(x[4 * i], x[4 * i + 1]), fmaxf(x[4 * i + 2], x[4 * i + 3])) < tf)) {
+                const int e = 4 * (v + i * ST + tid);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) part[k] += exp2f((x[4 * i + k] - m) * 1.4426950408889634f);
-        sum = (part[0] + part[1]) + (part[2] + part[3]);
-    }
-    sum = warp_sum(sum);
-    if (lane == 0) wsum[warp] = sum;
+                for (int k = 0; k < 4; ++k) {
+                    const unsigned o = key_of(fmaxf(x[4 * i + k], -INFINITY));               // what is no number ranks with -inf
+                    if (o >= t && e + k < e_hi) {
+                        const int at = atomicAdd(&listed, 1);
+                        if (at < CAP) list[at] = ((unsigned long long)o << 32) | (unsigned)(0xffffffffu - (unsigned)(e + k));
+                    }
+                }
+            }
+    };
+    auto block_high = [&](unsigned mine) -> unsigned {
+        const unsigned h = __reduce_max_sync(0xffffffffu, mine);
+        __syncthreads();
+        if (lane == 0) red_hi[warp] = h;
+        __syncthreads();
+        return __reduce_max_sync(0xffffffffu, red_hi[lane & (W - 1)]);
+    };
 
-    // a value that the slice's best all reach
-    const int count = e_hi - e_lo;
-    unsigned t = 0;
-    if (count > 2 * picks) t = reach(own_top, 0x007fffffu, ordered(m), picks);
-    if (own_top >= t) {
+    // An element's thread goes by its index alone, whatever the row's alignment: equal rows get equal sums, and their continuations
+    // are equals that go by index.
+    float x[4 * NV];
+    for (int v = v0, chunk = 0, stage = 0; v < v1; v += CHUNK, ++chunk, stage = stage + 1 == STAGES ? 0 : stage + 1) {
+        fetch(now, v + (STAGES - 1) * CHUNK, stage == 0 ? STAGES - 1 : stage - 1);
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 1) : "memory");
+        __syncwarp();
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int e = 4 * (v0 + i * ST + tid);
+            const float4* const from = ring + ((stage * NV + i) * W + warp) * 33 + lane;
+            float4 f = from[0];
+            if (now.shift) {
+                const float4 g = from[1];
+                f = now.shift == 1 ? make_float4(f.y, f.z, f.w, g.x) : now.shift == 2 ? make_float4(f.z, f.w, g.x, g.y) : make_float4(f.w, g.x, g.y, g.z);
+            }
+            x[4 * i] = f.x; x[4 * i + 1] = f.y; x[4 * i + 2] = f.z; x[4 * i + 3] = f.w;
+        }
+        __syncwarp();                                      // the stage is free
+        const float high = highest(x);
+        top = fmaxf(top, high);
+        chunk_top[chunk][tid] = high;
+        add_up(x, high);
+    }
+    next();
+    const unsigned own = key_of(top);
+    const int holders = min(ST, v1 - v0);                  // threads with an element of the slice
+    {
+        const unsigned lo = __reduce_min_sync(0xffffffffu, tid < holders ? own : 0xffffffffu);
+        if (lane == 0) red_lo[warp] = lo;
+    }
+    const unsigned key_m = block_high(own);
+    const float m = from_ordered(key_m);
+    if (count > 2 * picks) {
+        t = reach(own, holders >= picks ? __reduce_min_sync(0xffffffffu, red_lo[lane & (W - 1)]) : MINUS_INF, key_m, picks);
+        tf = from_ordered(t);
+    }
+    if (v1 - v0 <= CHUNK) {
+        if (own >= t) gather(x, v0);
+    } else {
+        // the few chunks of a thread in which something reaches t are read once more, a thread an element
+        for (int c = 0, v = v0; v < v1; ++c, v += CHUNK)
+            if (chunk_top[c][tid] >= tf) again[atomicAdd(&cell, 1)] = (unsigned short)(c * ST + tid);
+        __syncthreads();
+        const int elements = cell * (4 * NV);
+        constexpr int AT_ONCE = 8;                         // loads in flight together
+        for (int i0 = tid; i0 < elements; i0 += AT_ONCE * ST) {
+            float again_x[AT_ONCE];
+            int again_e[AT_ONCE];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const unsigned o = key_of(x[4 * i + k]);
-                if (o >= t && e + k < e_hi) {
-                    const int at = atomicAdd(&listed, 1);
-                    if (at < CAP) list[at] = ((unsigned long long)o << 32) | (unsigned)(0xffffffffu - (unsigned)(e + k));
+            for (int q = 0; q < AT_ONCE; ++q) {
+                const int i = i0 + q * ST;
+                again_e[q] = e_hi;
+                if (i < elements) {
+                    const int at = again[i / (4 * NV)], c = at / ST, j = i & (4 * NV - 1);
+                    again_e[q] = 4 * (v0 + c * CHUNK + (j >> 2) * ST + (at & (ST - 1))) + (j & 3);
+                }
+                again_x[q] = again_e[q] < e_hi ? row[again_e[q]] : 0.f;
+            }
+#pragma unroll
+            for (int q = 0; q < AT_ONCE; ++q) {
+                const unsigned o = key_of(fmaxf(again_x[q], -INFINITY));
+                if (again_e[q] < e_hi && o >= t) {
+                    const int to = atomicAdd(&listed, 1);
+                    if (to < CAP) list[to] = ((unsigned long long)o << 32) | (unsigned)(0xffffffffu - (unsigned)again_e[q]);
                 }
             }
         }
     }
-    __syncthreads();
-    if (tid == 0) {
-        double total = 0.0;
-        for (int w = 0; w < ST / 32; ++w) total += (double)wsum[w];
-        *mine_stat = SliceStat{total, m, 0};
+
+    double total = 0.0;
+    {
+        const float to = whole_ref(m);                     // (the threads' largest ref, where that is taken)
+        const float ws = warp_sum(sum * two_to(ref - to));
+        if (lane == 0) wsum[warp] = ws;
     }
+    if (__syncthreads_or(sum != sum) || by_difference(m)) {
+        // something is no number, or infinite, or very large: once more
+        float s = 0.f;
+        if (m > -INFINITY)
+            for (int e = e_lo + tid; e < e_hi; e += ST) {
+                const float v = fmaxf(row[e], -INFINITY);
+                s += m == INFINITY ? (v == INFINITY ? 1.f : 0.f)   // the weight lies on the infinite ones alone
+                                   : ex2(by_difference(m) ? (v - m) * L : fmaf(v, L, -whole_ref(m)));
+            }
+        s = warp_sum(s);
+        __syncthreads();
+        if (lane == 0) wsum[warp] = s;
+        __syncthreads();
+    }
+    if (tid == 0)
+#pragma unroll
+        for (int w = 0; w < W; ++w) total += (double)wsum[w];
+
     int n = listed;
     if (n > CAP) {
-        // too many reach t: the value of the last one that belongs, then the index up to which its equals do
-        unsigned lo = t, hi = ordered(m);                  // count(>= lo) >= picks, count(> hi) = 0
+        // too many reach t (equals, most of them): the value of the last one that belongs, then the index up to which its equals do
+        unsigned lo = t, hi = key_m;                       // count(>= lo) >= picks, count(> hi) = 0
         unsigned probe = lo + 1;                           // (most often the many are equal: asked first)
+        auto count_of = [&](auto belongs) -> int {
+            int mine = 0;
+            for (int e = e_lo + tid; e < e_hi; e += ST) mine += belongs(key_of(fmaxf(row[e], -INFINITY)), e);
+            return block_count(mine, &cell);
+        };
         while (lo < hi) {
-            int c = 0;
-#pragma unroll
-            for (int i = 0; i < 4 * NV; ++i) {
-                const int e = 4 * (v0 + (i >> 2) * ST + tid) + (i & 3);
-                c += key_of(x[i]) >= probe && e < e_hi;
-            }
-            if (block_count(c, &cell) >= picks) lo = probe;
+            if (count_of([&](unsigned o, int) { return o >= probe; }) >= picks) lo = probe;
             else hi = probe - 1;
             probe = lo + (hi - lo + 1) / 2;
         }
-        int c = 0;
-#pragma unroll
-        for (int i = 0; i < 4 * NV; ++i) {
-            const int e = 4 * (v0 + (i >> 2) * ST + tid) + (i & 3);
-            c += key_of(x[i]) > lo && e < e_hi;
-        }
-        const int equals = picks - block_count(c, &cell);   // at least 1 of those with the value itself, the lowest indices
-        int b_lo = e_lo, b_hi = e_hi;                       // smallest b with `equals` of them below it
+        const int equals = picks - count_of([&](unsigned o, int) { return o > lo; });         // at least 1: the lowest indices
+        int b_lo = e_lo, b_hi = e_hi;                      // smallest b with `equals` of them below it
         while (b_lo < b_hi) {
             const int b = b_lo + (b_hi - b_lo) / 2;
-            c = 0;
-#pragma unroll
-            for (int i = 0; i < 4 * NV; ++i) {
-                const int e = 4 * (v0 + (i >> 2) * ST + tid) + (i & 3);
-                c += key_of(x[i]) == lo && e < b;
-            }
-            if (block_count(c, &cell) >= equals) b_hi = b;
+            if (count_of([&](unsigned o, int e) { return o == lo && e < b; }) >= equals) b_hi = b;
             else b_lo = b + 1;
         }
         __syncthreads();
         if (tid == 0) listed = 0;
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4 * NV; ++i) {
-            const int e = 4 * (v0 + (i >> 2) * ST + tid) + (i & 3);
-            const unsigned o = key_of(x[i]);
-            if (o > lo ? e < e_hi : o == lo && e < b_lo) {
+        for (int e = e_lo + tid; e < e_hi; e += ST) {
+            const unsigned o = key_of(fmaxf(row[e], -INFINITY));
+            if (o > lo || (o == lo && e < b_lo)) {
                 const int at = atomicAdd(&listed, 1);
                 if (at < CAP) list[at] = ((unsigned long long)o << 32) | (unsigned)(0xffffffffu - (unsigned)e);
             }
@@ -211,60 +348,99 @@ beam_slices_kernel(const float* __restrict__ logits, long long ld, int vocab, co
         __syncthreads();
         n = min(listed, CAP);
     }
-    for (int i = n + tid; i < picks; i += ST) mine_best[i] = 0ull;          // fewer elements than picks
-    for (int i = warp; i < n; i += ST / 32) {
+    if (tid == 0) *mine_stat = SliceStat{total, m, n <= 2 * picks ? n : picks};
+    if (n <= 2 * picks) {
+        for (int i = tid; i < n; i += ST) mine_best[i] = list[i];
+        continue;
+    }
+    for (int i = warp; i < n; i += W) {
         const unsigned long long key = list[i];
         int rank = 0;
         for (int j = lane; j < n; j += 32) rank += list[j] > key;
         rank = __reduce_add_sync(0xffffffffu, rank);
         if (lane == 0 && rank < picks) mine_best[rank] = key;
     }
+    }
 }
 
-// One CTA a group.  An element of the pool is a row's, a slice's and a rank's; 0 where a slice had fewer.
+// One CTA a group.  Of the pool's 2 * picks places a slice, the slice's first n are filled.
 __global__ void __launch_bounds__(MT)
-beam_merge_kernel(const unsigned long long* __restrict__ best, const SliceStat* __restrict__ stat, const float* __restrict__ scores,
-                  int vocab, int beams, int slices, int picks, float* __restrict__ out_scores, int* __restrict__ out_rows,
-                  int* __restrict__ out_tokens) {
-    __shared__ double base[MAX_BEAMS];                     // scores[b] - log of the row's sum
+beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const float* scores,
+                  int vocab, int beams, int slices, int picks, float* out_scores, int* out_rows,
+                  int* out_tokens) {
+    __shared__ double base[MAX_BEAMS], so_far[MAX_BEAMS];  // log of the row's sum; its score
     __shared__ float row_top[MAX_BEAMS];
     __shared__ double l_score[CAP];
     __shared__ long long l_flat[CAP];
-    __shared__ unsigned wmax[MT / 32];
+    __shared__ SliceStat held[LISTS];
+    __shared__ unsigned wmax[MT / 32], wmin[MT / 32];
+    __shared__ unsigned long long best_of[MT / 32];
     __shared__ int cell, listed;
     const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) listed = 0;
     pdl_wait();
+    const int lists = beams * slices, room = 2 * picks;
+    const unsigned long long* keys = best + (size_t)g * lists * room;
+    const SliceStat* of = stat + (size_t)g * lists;
+    for (int l = tid; l < min(lists, LISTS); l += MT) held[l] = of[l];
+    __syncthreads();
+    auto stat_of = [&](int l) -> SliceStat { return l < LISTS ? held[l] : of[l]; };
     for (int b = warp; b < beams; b += MT / 32) {
-        const SliceStat* s = stat + ((size_t)g * beams + b) * slices;
         float m = -INFINITY;
-        for (int i = lane; i < slices; i += 32) m = fmaxf(m, s[i].m);
+        for (int i = lane; i < slices; i += 32) m = fmaxf(m, stat_of(b * slices + i).m);
         m = warp_max(m);
+        const float ref = whole_ref(m);
         double sum = 0.0;
-        for (int i = lane; i < slices; i += 32)
-            if (s[i].m > -INFINITY) sum += s[i].m == m ? s[i].sum : s[i].sum * exp((double)s[i].m - (double)m);
+        for (int i = lane; i < slices; i += 32) {
+            const SliceStat s = stat_of(b * slices + i);
+            if (s.m == -INFINITY) continue;
+            if (!by_difference(m)) {
+                if (!by_difference(s.m)) sum += s.sum * two_to(whole_ref(s.m) - ref);        // (else far below: nothing)
+            } else if (by_difference(s.m)) {
+                sum += s.m == m ? s.sum : s.sum * exp((double)s.m - (double)m);
+            } else {
+                sum += s.sum * exp(0.6931471805599453 * whole_ref(s.m) - (double)m);
+            }
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
+            // log of the row's sum; that L is not log2 e to the last bit acts as a factor of the logits, here of the largest
+            const double l = log(sum);
             row_top[b] = m;
-            base[b] = m == INFINITY ? (double)scores[(size_t)g * beams + b] - log(sum) : (double)m + log(sum);
+            so_far[b] = (double)scores[(size_t)g * beams + b];
+            base[b] = m == INFINITY      ? l
+                      : by_difference(m) ? (double)m + l
+                                         : l + 0.6931471805599453 * ref + (double)m * (1.0 - 0.6931471805599453 * (double)L);
         }
     }
     __syncthreads();
-    // rank by rank, so that neighbouring threads hold the heads of the lists
-    const int lists = beams * slices, pool = lists * picks;
-    const unsigned long long* keys = best + (size_t)g * pool;
-    auto key_at = [&](int i, int& b) -> unsigned long long {
-        const int rank = i / lists, list = i - rank * lists;
-        b = list / slices;
-        return keys[(size_t)list * picks + rank];
+    // every element of the pool once: a warp four lists, whose loads are in flight together
+    auto each = [&](auto use) {
+        constexpr int AT_ONCE = 4;
+        for (int l0 = warp; l0 < lists; l0 += AT_ONCE * (MT / 32)) {
+            int n[AT_ONCE], most = 0;
+#pragma unroll
+            for (int q = 0; q < AT_ONCE; ++q) {
+                const int l = l0 + q * (MT / 32);
+                n[q] = l < lists ? stat_of(l).n : 0;
+                most = max(most, n[q]);
+            }
+            for (int k = lane; k < most; k += 32) {
+                unsigned long long key[AT_ONCE];
+#pragma unroll
+                for (int q = 0; q < AT_ONCE; ++q) key[q] = k < n[q] ? keys[(size_t)(l0 + q * (MT / 32)) * room + k] : 0ull;
+#pragma unroll
+                for (int q = 0; q < AT_ONCE; ++q)
+                    if (key[q]) use((l0 + q * (MT / 32)) / slices, key[q]);
+            }
+        }
     };
     // the element's score; -inf for what is no number (a row all of whose logits are -inf)
     auto score_of = [&](int b, unsigned long long key) -> double {
-        const float x = from_ordered((unsigned)(key >> 32)), m = row_top[b];
-        double v;
-        if (m == INFINITY) v = x == INFINITY ? base[b] : -INFINITY;
-        else v = x == -INFINITY ? -INFINITY : (double)scores[(size_t)g * beams + b] + ((double)x - base[b]);
+        const float x = from_ordered((unsigned)(key >> 32));
+        double v = so_far[b] + ((double)x - base[b]);
+        if (row_top[b] == INFINITY) v = x == INFINITY ? so_far[b] - base[b] : -INFINITY;
         return v == v ? v : -INFINITY;
     };
     auto flat_of = [&](int b, unsigned long long key) -> long long {
@@ -272,27 +448,21 @@ beam_merge_kernel(const unsigned long long* __restrict__ best, const SliceStat* 
     };
     // 32-bit keys for the search: rounding keeps the order, and equals after rounding are all gathered
     unsigned mine = 0;
-    for (int i = tid; i < pool; i += MT) {
-        int b;
-        const unsigned long long key = key_at(i, b);
-        if (key) mine = max(mine, ordered((float)score_of(b, key)));
-    }
+    each([&](int b, unsigned long long key) { mine = max(mine, ordered((float)score_of(b, key))); });
     unsigned top = __reduce_max_sync(0xffffffffu, mine);
-    if (lane == 0) wmax[warp] = top;
-    __syncthreads();
+    const unsigned low = __reduce_min_sync(0xffffffffu, mine ? mine : 0xffffffffu);
+    if (lane == 0) { wmax[warp] = top; wmin[warp] = low; }
+    const int holders = __syncthreads_count(mine != 0);
     top = __reduce_max_sync(0xffffffffu, wmax[lane & (MT / 32 - 1)]);
-    unsigned t = 1;
-    if (pool > 2 * picks) t = reach(mine, 1, top, picks);
-    for (int i = tid; i < pool; i += MT) {
-        int b;
-        const unsigned long long key = key_at(i, b);
-        if (!key) continue;
+    unsigned t = holders >= picks ? __reduce_min_sync(0xffffffffu, wmin[lane & (MT / 32 - 1)]) : 1;
+    if (lists > 1) t = reach(mine, t, top, picks);
+    each([&](int b, unsigned long long key) {
         const double s = score_of(b, key);
         if (ordered((float)s) >= t) {
             const int at = atomicAdd(&listed, 1);
             if (at < CAP) { l_score[at] = s; l_flat[at] = flat_of(b, key); }
         }
-    }
+    });
     __syncthreads();
     int n = listed;
     if (n > CAP) {
@@ -303,18 +473,28 @@ beam_merge_kernel(const unsigned long long* __restrict__ best, const SliceStat* 
         };
         auto count_of = [&](auto belongs) -> int {
             int c = 0;
-            for (int i = tid; i < pool; i += MT) {
-                int b;
-                const unsigned long long key = key_at(i, b);
-                if (key) c += belongs(ordered64(score_of(b, key) + 0.0), flat_of(b, key));
-            }
+            each([&](int b, unsigned long long key) { c += belongs(ordered64(score_of(b, key) + 0.0), flat_of(b, key)); });
             return block_count(c, &cell);
         };
-        unsigned long long lo = 0, hi = ~0ull;
+        // asked first: whether it is -inf (most words forbidden), or all are equals of the best (the next of two probes)
+        unsigned long long lo = ordered64(-INFINITY), hi = ~0ull, probe = lo + 1;
+        bool best_next = true;
         while (lo < hi) {
-            const unsigned long long mid = lo + (hi - lo) / 2 + 1;
-            if (count_of([&](unsigned long long o, long long) { return o >= mid; }) >= picks) lo = mid;
-            else hi = mid - 1;
+            if (count_of([&](unsigned long long o, long long) { return o >= probe; }) >= picks) lo = probe;
+            else hi = probe - 1;
+            probe = lo + (hi - lo) / 2 + 1;
+            if (best_next && lo < hi) {
+                unsigned long long most = 0;
+                each([&](int b, unsigned long long key) { most = max(most, ordered64(score_of(b, key) + 0.0)); });
+                const unsigned high = __reduce_max_sync(0xffffffffu, (unsigned)(most >> 32));
+                const unsigned low = __reduce_max_sync(0xffffffffu, (unsigned)(most >> 32) == high ? (unsigned)most : 0u);
+                __syncthreads();
+                if (lane == 0) best_of[warp] = (unsigned long long)high << 32 | low;
+                __syncthreads();
+                for (int w = 0; w < MT / 32; ++w) most = max(most, best_of[w]);
+                hi = probe = most;
+            }
+            best_next = false;
         }
         const int equals = picks - count_of([&](unsigned long long o, long long) { return o > lo; });
         long long f_lo = 0, f_hi = (long long)beams * vocab;
@@ -326,10 +506,7 @@ beam_merge_kernel(const unsigned long long* __restrict__ best, const SliceStat* 
         __syncthreads();
         if (tid == 0) listed = 0;
         __syncthreads();
-        for (int i = tid; i < pool; i += MT) {
-            int b;
-            const unsigned long long key = key_at(i, b);
-            if (!key) continue;
+        each([&](int b, unsigned long long key) {
             const double s = score_of(b, key);
             const unsigned long long o = ordered64(s + 0.0);
             const long long f = flat_of(b, key);
@@ -337,7 +514,7 @@ beam_merge_kernel(const unsigned long long* __restrict__ best, const SliceStat* 
                 const int at = atomicAdd(&listed, 1);
                 if (at < CAP) { l_score[at] = s; l_flat[at] = f; }
             }
-        }
+        });
         __syncthreads();
         n = min(listed, CAP);
     }
@@ -358,16 +535,17 @@ beam_merge_kernel(const unsigned long long* __restrict__ best, const SliceStat* 
 
 int vectors_of(int vocab) { return (vocab + 3) / 4; }
 
-// 16-byte loads a thread: as many as leave two CTAs an SM something to do.  Few rows go in more and smaller slices
-int vectors_a_thread(int rows, int vocab, int sms) {
-    const int n = vectors_of(vocab);
-    for (int nv = 8; nv > 2; nv >>= 1)
-        if ((long long)rows * ((n + nv * ST - 1) / (nv * ST)) >= 2ll * sms) return nv;
-    return 2;
-}
+// Slices a row: what takes the fewest rounds of chunks, all CTAs at work, a slice's end costing about what two chunks' way does
 int slices_of(int rows, int vocab, int sms) {
-    const int a_slice = vectors_a_thread(rows, vocab, sms) * ST;
-    return (vectors_of(vocab) + a_slice - 1) / a_slice;
+    const int n = vectors_of(vocab), chunks = (n + NV * ST - 1) / (NV * ST);
+    int best = chunks;
+    long long best_cost = -1;
+    for (int s = (chunks + MAX_CHUNKS - 1) / MAX_CHUNKS; s <= chunks; s = s < 64 ? s + 1 : 2 * s) {
+        const int a_slice = (n + s - 1) / s, of_slice = (a_slice + NV * ST - 1) / (NV * ST);
+        const long long rounds = ((long long)rows * s + CTAS * sms - 1) / (CTAS * sms), cost = rounds * (of_slice + 2);
+        if (of_slice <= MAX_CHUNKS && (best_cost < 0 || cost < best_cost)) { best = s; best_cost = cost; }
+    }
+    return best;
 }
 }  // namespace
 
@@ -380,14 +558,15 @@ RI_API int ri_beam_select(const float* logits, long long ld, int vocab, const fl
     if (beams < 1 || beams > MAX_BEAMS || picks < 1 || picks > MAX_PICKS || vocab < 1 || vocab > (1 << 30) ||
         (long long)beams * vocab < picks || (long long)groups * beams > 65535)
         return (int)cudaErrorInvalidValue;
-    const int rows = groups * beams, nv = vectors_a_thread(rows, vocab, sms), slices = slices_of(rows, vocab, sms);
+    const int rows = groups * beams, slices = slices_of(rows, vocab, sms);
     const int a_slice = (vectors_of(vocab) + slices - 1) / slices;
     SliceStat* stat = (SliceStat*)scratch;
     unsigned long long* best = (unsigned long long*)(stat + (size_t)rows * slices);
-    const dim3 grid(slices, rows);
     cudaStream_t s = (cudaStream_t)stream;
-    auto kernel = nv == 8 ? beam_slices_kernel<8> : nv == 4 ? beam_slices_kernel<4> : beam_slices_kernel<2>;
-    RI_CHECKED(ri_launch(kernel, grid, dim3(ST), 0, s, logits, ld, vocab, scores, picks, a_slice, best, stat));
+    constexpr int ring = STAGES * NV * (ST / 32) * 33 * 16;
+    RI_CHECKED((int)cudaFuncSetAttribute(beam_slices_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring));
+    RI_CHECKED(ri_launch(beam_slices_kernel, dim3(min(rows * slices, CTAS * sms)), dim3(ST), ring, s, logits, ld, vocab, scores, picks, rows * slices,
+                         slices, a_slice, best, stat));
     RI_CHECKED(ri_launch(beam_merge_kernel, dim3(groups), dim3(MT), 0, s, best, stat, scores, vocab, beams, slices, picks, out_scores, out_rows,
                          out_tokens));
     return ri_launch_status();

@@ -2071,8 +2071,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, out_scor
     if R > 65535 or V > 1 << 30:
         raise KernelError(f"beam_select: {R} rows of {V} tokens (up to 65,535 rows and 2^30 tokens)")
     lib, sms = L.beams(), L.num_sms(logits.device)
-    # a sum (16 bytes) and the best (8 each) of every slice of every row
-    scratch = torch.empty(R * lib.ri_beam_select_slices(R, V, sms) * (2 + picks), dtype=torch.int64, device=logits.device)
+    # a sum (16 bytes) and the best (8 each, twice `picks` at most) of every slice of every row
+    scratch = torch.empty(R * lib.ri_beam_select_slices(R, V, sms) * (2 + 2 * picks), dtype=torch.int64, device=logits.device)
     check(lib.ri_beam_select(_p(logits), logits.stride(0), V, _p(scores), groups, beams, picks, sms, _p(scratch), _p(out_scores), _p(out_rows),
                              _p(out_tokens), stream_ptr()), "beam_select", 2)
 
