@@ -7,6 +7,12 @@ pages back as soon as the window has passed them.  A fixed-state group (`FixedSt
 keeps one row per request slot.  Every request holds one slot while it is live, whether
 or not the architecture has fixed state.
 
+Requests can be forked (`fork`): the copies share the pages that are full, whose holders the pool
+counts, and own what is still written to (the page the next token goes to, the state slot).  In a
+family of equal length every member can take over what another one has (`reorder`), and the pages
+that are held can be moved to the lowest numbers (`compact`).  All three say what has to be copied
+on the device.
+
 This is host bookkeeping only; the device tensors belong to `CacheStorage`.  In the
 reference every layer is full attention over one shared block-id space
 (crates/infer-core/src/kv.rs:41-70) and per-request tables are host vectors
@@ -81,11 +87,13 @@ class Lease:
     def __init__(self, manager: "CacheManager", batch: List[Tuple[Any, int]], taken: List[Dict[int, int]]):
         self._m, self._batch, self._taken = manager, batch, taken
         self.settled = False
+        manager._leases += 1
 
     def _settle(self) -> None:
         if self.settled:
             raise RuntimeError("this lease was already committed or released")
         self.settled = True
+        self._m._leases -= 1
 
     def commit(self) -> None:
         self._settle()
@@ -132,6 +140,29 @@ class _Request:
     length: int = 0
     tables: Dict[int, List[int]] = field(default_factory=dict)     # group -> page per position block (-1: given back)
     first_live: Dict[int, int] = field(default_factory=dict)       # group -> first block still held
+    family: int = 0                                                # uid of the request it was first forked from (its own: none)
+    common: int = 1 << 60                                          # any two of a family share at least the lesser of theirs
+    changes: int = 0                                               # how often `reorder` has changed the tables
+    settled: Dict[int, int] = field(default_factory=dict)          # group -> leading blocks that no `reorder` has changed
+
+
+@dataclass
+class DeviceCopies:
+    """What a fork or a reorder has to move on the device.  `pages`: group -> [(source, destination)], the
+    first `tokens` tokens of each; `slots`: [(source, destination)]."""
+    pages: Dict[int, List[Tuple[int, int]]]
+    slots: List[Tuple[int, int]]
+    tokens: int
+
+
+@dataclass
+class DeviceReorder:
+    """A reorder: entry r of each list takes over what entry parents[r] has.  `pages`: group -> the page every member
+    writes to next, of which the first `tokens` tokens are in use (empty where none is)."""
+    parents: List[int]
+    slots: List[int]
+    pages: Dict[int, List[int]]
+    tokens: int
 
 
 class CacheManager:
@@ -148,6 +179,7 @@ class CacheManager:
         self.slots = StateSlots(max_requests)
         self._req: Dict[Any, _Request] = {}
         self._opened = 0
+        self._leases = 0                           # leases that are neither committed nor released
         self.newly_opened_slots: List[int] = []    # slots whose fixed state must be zeroed before use
 
     # ----------------------------------------------------------------- life of a request
@@ -157,7 +189,7 @@ class CacheManager:
         slot = self.slots.take()
         self._opened += 1
         self._req[request_id] = _Request(slot, self._opened, 0, {g: [] for g in self.pools},
-                                         {g: 0 for g in self.pools})
+                                         {g: 0 for g in self.pools}, family=self._opened)
         self.newly_opened_slots.append(slot)
         return slot
 
@@ -182,6 +214,115 @@ class CacheManager:
         for g, table in r.tables.items():
             self.pools[g].free(p for p in table if p >= 0)
         self.slots.give_back(r.slot)
+
+    # ------------------------------------------------------------------ forks of a request
+    def _no_lease(self, what: str) -> None:
+        if self._leases:
+            raise RuntimeError(f"{what} while a step's lease is out")
+
+    def fork_needs(self, request_id: Any, copies: int) -> Dict[int, int]:
+        """Pages each group hands out for so many forks of a request: its page that is partly filled, once a fork."""
+        part = self._req[request_id].length % self.page_size != 0
+        return {g: copies if part else 0 for g in self.pools}
+
+    def fork(self, request_id: Any, new_ids: Sequence[Any]) -> DeviceCopies:
+        """Opens `new_ids` as copies of a request: they share its full pages and get a page of their own for the one
+        that is partly filled, and a state slot.  All or nothing (`OutOfPages`, `OutOfSlots`, KeyError for an id that is
+        open)."""
+        self._no_lease("fork")
+        r = self._req[request_id]
+        new_ids = list(new_ids)
+        if len(set(new_ids)) != len(new_ids) or any(i in self._req for i in new_ids):
+            raise KeyError(f"fork: an id of {new_ids!r} is open already, or stands there twice")
+        if len(new_ids) > self.slots.free_count:
+            raise OutOfSlots(f"{len(new_ids)} forks, {self.slots.free_count} free request slots")
+        for g, k in self.fork_needs(request_id, len(new_ids)).items():
+            if k > self.pools[g].free_count:
+                raise OutOfPages(k, self.pools[g].free_count, g)
+        full, used = divmod(r.length, self.page_size)
+        copies = DeviceCopies({g: [] for g in self.pools}, [], used)
+        r.common = min(r.common, r.length)
+        for i in new_ids:
+            slot = self.slots.take()
+            self._opened += 1
+            tables = {}
+            for g, pool in self.pools.items():
+                tables[g] = r.tables[g][:full]
+                pool.share(p for p in tables[g] if p >= 0)
+                if used:
+                    (page,) = pool.alloc(1)
+                    copies.pages[g].append((r.tables[g][full], page))
+                    tables[g].append(page)
+            self._req[i] = _Request(slot, self._opened, r.length, tables, dict(r.first_live), family=r.family, common=r.common)
+            copies.slots.append((r.slot, slot))
+            if r.slot in self.newly_opened_slots:          # nothing in it yet: zeroed like the other one's
+                self.newly_opened_slots.append(slot)
+        return copies
+
+    def common_length(self, request_ids: Sequence[Any]) -> int:
+        """Tokens at the start that these requests certainly share (0 for requests of several families)."""
+        reqs = [self._req[i] for i in request_ids]
+        if any(r.family != reqs[0].family for r in reqs):
+            return 0
+        return min(min(r.common, r.length) for r in reqs)
+
+    def reorder(self, request_ids: Sequence[Any], parents: Sequence[int]) -> DeviceReorder:
+        """Request r takes over what request parents[r] holds, all at once; any mapping.  The requests are of one family and of
+        equal length.  Full pages change holders; the page that is partly filled and the state slot stay whose they are, and
+        their content moves."""
+        self._no_lease("reorder")
+        reqs = [self._req[i] for i in request_ids]
+        if len(parents) != len(reqs) or any(not 0 <= p < len(reqs) for p in parents) or len(set(request_ids)) != len(reqs):
+            raise ValueError(f"reorder: {len(reqs)} requests and the parents {list(parents)!r}")
+        if any(r.length != reqs[0].length or r.family != reqs[0].family for r in reqs):
+            raise ValueError("reorder: the requests are not of one family and one length")
+        full, used = divmod(reqs[0].length, self.page_size) if reqs else (0, 0)
+        out = DeviceReorder([int(p) for p in parents], [r.slot for r in reqs], {}, used)
+        for g, pool in self.pools.items():
+            fresh = []
+            for r, p in zip(reqs, parents):
+                mine, theirs = r.tables[g], reqs[p].tables[g]
+                if mine is theirs:
+                    continue
+                at = next((b for b, (x, y) in enumerate(zip(mine[:full], theirs[:full])) if x != y), full)
+                if at < full:
+                    fresh.append((r, at, theirs[at:full]))
+            for _r, _at, pages in fresh:                   # everyone's new pages before anyone's old ones are given back
+                pool.share(p for p in pages if p >= 0)
+            for r, at, pages in fresh:
+                pool.free(p for p in r.tables[g][at:full] if p >= 0)
+                r.tables[g][at:full] = pages
+                r.settled[g] = min(at, r.settled.get(g, at))
+                r.changes += 1
+            out.pages[g] = [r.tables[g][full] for r in reqs] if used else []
+        common = [r.common for r in reqs]
+        for r, p in zip(reqs, parents):
+            r.common = common[p]
+        return out
+
+    def changes(self, request_id: Any) -> Tuple[int, Dict[int, int]]:
+        """How often the tables were changed other than by new pages, and the leading blocks of each that never were."""
+        r = self._req[request_id]
+        return r.changes, r.settled
+
+    def compact(self) -> Dict[int, List[Tuple[int, int]]]:
+        """Moves the pages that are held to the lowest numbers of their pools: group -> [(from, to)], to be copied on the
+        device before anything else is written there."""
+        self._no_lease("compact")
+        out: Dict[int, List[Tuple[int, int]]] = {}
+        for g, pool in self.pools.items():
+            moves = pool.compact()
+            out[g] = sorted(moves.items())
+            if moves:
+                for r in self._req.values():
+                    table = r.tables[g]
+                    hit = [b for b, p in enumerate(table) if p in moves]
+                    for b in hit:
+                        table[b] = moves[table[b]]
+                    if hit:
+                        r.settled[g] = min(hit[0], r.settled.get(g, hit[0]))
+                        r.changes += 1
+        return out
 
     # -------------------------------------------------------------------------- pages
     def _blocks_for(self, length: int) -> int:
@@ -258,18 +399,22 @@ class CacheManager:
 
     # --------------------------------------------------------------------- self-check
     def check_invariants(self) -> None:
-        """No page lost, held twice, or both held and free; no slot shared."""
+        """No page lost, held by more than it counts, written to by two, or both held and free; no slot shared."""
         for g, pool in self.pools.items():
-            held: List[int] = []
+            holders: Dict[int, int] = {}
             for r in self._req.values():
-                held.extend(p for p in r.tables[g] if p >= 0)
-            if len(held) != len(set(held)):
-                raise AssertionError(f"group {g}: a page is held twice")
+                for b, p in enumerate(r.tables[g]):
+                    if p >= 0:
+                        holders[p] = holders.get(p, 0) + 1
+                        if holders[p] > 1 and (b + 1) * self.page_size > r.length:
+                            raise AssertionError(f"group {g}: a page that is written to is held twice")
+            if any(pool.holders(p) != n for p, n in holders.items()):
+                raise AssertionError(f"group {g}: a page is held by another number than it counts")
             free = pool.free_set()
-            if free & set(held):
+            if free & set(holders):
                 raise AssertionError(f"group {g}: a page is both held and free")
-            if len(free) + len(held) != pool.num_pages:
-                raise AssertionError(f"group {g}: {pool.num_pages - len(free) - len(held)} pages lost")
+            if len(free) + len(holders) != pool.num_pages:
+                raise AssertionError(f"group {g}: {pool.num_pages - len(free) - len(holders)} pages lost")
         slots = [r.slot for r in self._req.values()]
         if len(slots) != len(set(slots)):
             raise AssertionError("a state slot is shared")

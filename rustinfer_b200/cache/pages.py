@@ -6,11 +6,15 @@ all-or-nothing.  RustInfer's `GlobalKvAllocator` keeps the same contract over to
 crates/infer-worker/src/domain/global_kv_alloc.rs:56-71,129-194).  Where the reference
 ignores a double free with a warning, this pool raises: a page freed twice is a fault of
 the caller that must not pass silently.
+
+A page may have several holders: requests that were forked from one another share the pages that
+are full.  `share` adds a holder, `free` takes one away, and the page is free again when the last
+is gone.
 """
 from __future__ import annotations
 
 import heapq
-from typing import Iterable, List
+from typing import Dict, Iterable, List
 
 
 class OutOfPages(RuntimeError):
@@ -29,7 +33,7 @@ class PagePool:
             raise ValueError("a page pool needs at least one page")
         self.num_pages = num_pages
         self._free: List[int] = list(range(num_pages))      # a heap; sorted is a valid heap
-        self._is_free = [True] * num_pages
+        self._holders = [0] * num_pages
 
     @property
     def free_count(self) -> int:
@@ -45,18 +49,41 @@ class PagePool:
         else:
             out = [heapq.heappop(self._free) for _ in range(n)]
         for p in out:
-            self._is_free[p] = False
+            self._holders[p] = 1
         return out
 
+    def share(self, pages: Iterable[int]) -> None:
+        """One more holder for each of `pages`, which someone holds."""
+        holders = self._holders
+        for p in pages:
+            if not 0 <= p < self.num_pages or holders[p] == 0:
+                raise ValueError(f"page {p} is held by nobody")
+            holders[p] += 1
+
     def free(self, pages: Iterable[int]) -> None:
-        free, is_free, most = self._free, self._is_free, self.num_pages
+        free, holders, most = self._free, self._holders, self.num_pages
         for p in pages:
             if not 0 <= p < most:
                 raise ValueError(f"page {p} is outside the pool of {self.num_pages}")
-            if is_free[p]:
+            n = holders[p]
+            if n == 0:
                 raise ValueError(f"page {p} freed twice")
-            is_free[p] = True
-            heapq.heappush(free, p)
+            holders[p] = n - 1
+            if n == 1:
+                heapq.heappush(free, p)
+
+    def holders(self, page: int) -> int:
+        return self._holders[page]
+
+    def compact(self) -> Dict[int, int]:
+        """Held pages take the lowest numbers: {old: new} of the ones that move (each to a number that was free)."""
+        held = self.num_pages - len(self._free)
+        to = sorted(p for p in self._free if p < held)
+        moves = dict(zip((p for p in range(held, self.num_pages) if self._holders[p]), to))
+        for old, new in moves.items():
+            self._holders[new], self._holders[old] = self._holders[old], 0
+        self._free = list(range(held, self.num_pages))
+        return moves
 
     def free_set(self) -> set:
         return set(self._free)

@@ -47,6 +47,17 @@ def _run(path: str) -> int:
     if not prompts:
         raise SystemExit("the run file has no [[request]] table")
     s = dict(cfg.sampling)
+    beams = int(s.get("beams", 1))
+    if beams > 1:
+        from .engine.beam import BeamParams
+        found = engine.beam_search(prompts, BeamParams(
+            beams=beams, best=int(s.get("best", 1)), max_tokens=int(s.get("max_tokens", 16)), length_penalty=float(s.get("length_penalty", 1.0)),
+            early_stopping=bool(s.get("early_stopping", False)), ignore_eos=bool(s.get("ignore_eos", cfg.ignore_eos))))
+        for i, (prompt, hyps) in enumerate(zip(prompts, found)):
+            for h in hyps:
+                print(json.dumps({"request": i, "prompt_tokens": len(prompt), "tokens": h.tokens, "finish_reason": h.finish_reason,
+                                  "log_prob": h.log_prob, "score": h.score}))
+        return _end(engine, scratch)
     params = SamplingParams(temperature=float(s.get("temperature", 0.0)), top_k=int(s.get("top_k", 0)),
                             top_p=float(s.get("top_p", 1.0)), min_p=float(s.get("min_p", 0.0)),
                             seed=s.get("seed"), max_tokens=int(s.get("max_tokens", 16)),
@@ -54,6 +65,10 @@ def _run(path: str) -> int:
     for res in engine.generate(prompts, params):
         print(json.dumps({"request": res.request_id, "prompt_tokens": len(res.prompt),
                           "tokens": res.tokens, "finish_reason": res.finish_reason}))
+    return _end(engine, scratch)
+
+
+def _end(engine, scratch) -> int:
     st = engine.stats
     print(json.dumps({"steps": st.steps, "prompt_tokens": st.prompt_tokens,
                       "generated_tokens": st.generated_tokens, "preemptions": st.preemptions,

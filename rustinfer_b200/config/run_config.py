@@ -6,7 +6,8 @@ accepted and ignored, so that a reference run file loads; `model_type` never sta
 here, it always comes from config.json.
 
 Added for this engine: `dtype`, a `[sampling]` table (temperature, top_k, top_p, min_p,
-seed, max_tokens), `[[request]]` tables (`prompt_ids` or `random_len`) and a
+seed, max_tokens; with `beams` above 1 beam search instead, and then best,
+length_penalty, early_stopping), `[[request]]` tables (`prompt_ids` or `random_len`) and a
 `[random_weights]` table (`config`, `seed`, `std`) that builds the model folder first.
 """
 from __future__ import annotations

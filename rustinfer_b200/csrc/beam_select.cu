@@ -405,6 +405,8 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
+            // the largest weight as it is, not to the 2 ulp of its exponential: a token that is all but certain costs nothing
+            if (!by_difference(m)) sum += exp2((double)m * (double)L - (double)ref) - (double)ex2(fmaf(m, L, -ref));
             // log of the row's sum; that L is not log2 e to the last bit acts as a factor of the logits, here of the largest
             const double l = log(sum);
             row_top[b] = m;

@@ -2,6 +2,7 @@
 
     engine = Engine(model="path/to/folder", dtype="bfloat16", max_batch_seqs=32, ...)
     results = engine.generate([[1, 2, 3], [4, 5]], SamplingParams(max_tokens=16))
+    best = engine.beam_search([[1, 2, 3], [4, 5]], BeamParams(beams=4, max_tokens=16))
 
 Options carry RustInfer's names and meanings (run file keys,
 crates/infer-protocol/src/config.rs:55-262).  The reference has no Python entry point
@@ -21,6 +22,7 @@ import torch
 from ..config.run_config import DEFAULT_CAPTURE_SIZES, RunConfig
 from ..sampling.params import SamplingParams
 from ..sampling.sampler import Sampler, fresh_seed
+from .beam import BeamHypothesis, BeamParams, BeamSearch
 from .runner import ModelRunner, StepEntry
 from ..ops import kernels as K
 from .scheduler import FINISHED, Request, Scheduler
@@ -263,3 +265,22 @@ class Engine:
         self.stats.seconds += time.perf_counter() - t0
         self.runner.check_kernel_errors()
         return [self.take_finished(i) for i in ids]
+
+    # --------------------------------------------------------------------- beam search
+    def beam_search(self, prompts: Sequence[Sequence[int]], params: Optional[BeamParams] = None) -> List[List[BeamHypothesis]]:
+        """The best continuations of every prompt (lists of token ids on the host): for each prompt up to `params.best`
+        hypotheses, best first.  Runs to the end by itself; no request may be under way."""
+        if self.has_unfinished():
+            raise RuntimeError("beam search needs the engine to itself: there are requests under way")
+        p = params or BeamParams()
+        if self.ignore_eos and not p.ignore_eos:
+            p = BeamParams(**{**p.__dict__, "ignore_eos": True})
+        t0 = time.perf_counter()
+        search = BeamSearch(self.runner, p, self.runner.spec.eos_token_ids)
+        out = search.run([[int(t) for t in q] for q in prompts])
+        self.stats.steps += search.steps
+        self.stats.prompt_tokens += sum(len(q) for q in prompts)
+        self.stats.generated_tokens += sum(len(h.tokens) for hyps in out for h in hyps)
+        self.stats.seconds += time.perf_counter() - t0
+        self.runner.check_kernel_errors()
+        return out

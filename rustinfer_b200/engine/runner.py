@@ -27,6 +27,7 @@ from ..cache.manager import CacheLayout, CacheManager
 from ..cache.pages import OutOfPages
 from ..config.registry import load_model_description
 from ..models.decoder import Decoder
+from ..ops import kernels as _k
 from ..ops.library import read_stream_budget
 from ..parts.base import (BuildContext, FixedState, GroupStep, HostEntry, PagedKV, PagedLayerCache,
                           StateLayerCache, StepContext, StepShape)
@@ -98,20 +99,23 @@ class _DecodeGraph:
     of page 0 and writes nothing (RustInfer pads with one-token rows on a scratch block,
     crates/infer-worker/src/application/worker_scheduler.rs:685-718)."""
 
-    def __init__(self, runner: "ModelRunner", bucket: int):
+    def __init__(self, runner: "ModelRunner", bucket: int, beams: int = 0):
         self.bucket = bucket
+        self.beams = beams
         P = runner.max_pages_per_request
         groups = runner.layout.paged_groups()
         self.spare_slot = runner.max_batch_seqs               # the state row padding rows point at
         # what the parts' index arrays look like for `bucket` rows of one token each
         shape = self._shape(np.zeros(bucket, dtype=np.int64), np.full(bucket, self.spare_slot, dtype=np.int64))
         built = [(need, need.build(shape)) for need in runner.index_needs]
-        # fixed layout: token_ids, positions, cu_q, kv_len, slots, rows, [table, slot_of_token]*, index arrays
+        # fixed layout: token_ids, positions, cu_q, kv_len, slots, rows, [table, slot_of_token]*, index arrays, shared lengths of beams
         sizes = [bucket, bucket, bucket + 1, bucket, bucket, bucket]
         for _ in groups:
             sizes += [bucket * P, bucket]
         for _need, arrays in built:
             sizes += [int(a.size) for a in arrays]
+        if beams > 1:
+            sizes.append(bucket // beams)
         self.offsets = []
         at = 0
         for n in sizes:
@@ -123,6 +127,7 @@ class _DecodeGraph:
         self.event: Optional[torch.cuda.Event] = None
         self.row_owner: List[Any] = [None] * bucket          # uid of the request whose table sits in a row
         self.row_pages: List[List[int]] = [[0] * len(groups) for _ in range(bucket)]
+        self.row_changes = [0] * bucket                      # how often that request's table had been changed when it was written
         v = [self.dev[o: o + n] for o, n in self.offsets]
         hv = [self.hv[o: o + n] for o, n in self.offsets]
         self.h_tokens, self.h_pos, h_cu, self.h_kv, self.h_slots, h_rows = hv[:6]
@@ -151,11 +156,13 @@ class _DecodeGraph:
             indices[need.key] = tuple(devs)
             if need.depends_on_positions:
                 self.moving_indices.append((need, hosts))
+        self.h_shared = hv[-1] if beams > 1 else None
         self.dev.copy_(self.host)
         self.step = StepContext(
             num_tokens=bucket, num_entries=bucket, token_ids=v[0], positions=v[1], cu_q=v[2], kv_len=v[3],
             state_slots=v[4], groups=gsteps, entries=[], max_q_len=1,
-            max_kv_len=runner.max_model_len, decode_only=True, indices=indices)
+            max_kv_len=runner.max_model_len, decode_only=True, indices=indices,
+            beams=beams, shared_len=v[-1] if beams > 1 else None, max_own_len=min(256, runner.max_model_len) if beams > 1 else 0)
         self.rows = v[5]
         # one eager run (libraries pick their algorithms, lazy kernels get built), then capture
         torch.cuda.synchronize()
@@ -210,6 +217,12 @@ class _DecodeGraph:
             if self.row_owner[i] != uid:
                 self.row_owner[i] = uid
                 self.row_pages[i] = [0] * len(groups)
+                self.row_changes[i] = cache.changes(rid)[0]
+            else:
+                changes, settled = cache.changes(rid)
+                if self.row_changes[i] != changes:           # a reorder or a compaction: written again from where it may differ
+                    self.row_changes[i] = changes
+                    self.row_pages[i] = [min(n, settled.get(g, n)) for n, g in zip(self.row_pages[i], groups)]
             for gi, g in enumerate(groups):
                 table = cache.block_table(rid, g)
                 start, n = self.row_pages[i][gi], len(table)
@@ -222,6 +235,11 @@ class _DecodeGraph:
                 if page < 0:
                     raise StepError("a token would be written to a page that was given back")
                 self.h_slot_of_token[gi][i] = page * ps + pos % ps
+        if self.h_shared is not None:
+            k = self.beams
+            for j in range(self.bucket // k):
+                rows = [e.request_id for e in entries[j * k: (j + 1) * k]]
+                self.h_shared[j] = cache.common_length(rows) if len(rows) == k else 0
         for i in range(len(entries), self.bucket):           # padding rows
             if self.row_owner[i] is not None:
                 self.row_owner[i] = None
@@ -304,7 +322,7 @@ class ModelRunner:
         self.steps_run = 0
         self.h2d_bytes_last = 0
         self.graph_replays = 0
-        self._graphs: Dict[int, "_DecodeGraph"] = {}
+        self._graphs: Dict[Any, "_DecodeGraph"] = {}          # by rows; by (rows, beams a request) of steps of beams
         self._graph_pool = None
         self.use_graphs = bool(self.capture_sizes) and self.model.graph_safe
 
@@ -380,6 +398,69 @@ class ModelRunner:
     def close(self, request_id: Any) -> None:
         self.cache.close(request_id)
 
+    def _i32(self, values: Sequence[int]) -> torch.Tensor:
+        return torch.tensor(list(values), dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
+
+    def fork(self, request_id: Any, new_ids: Sequence[Any]) -> None:
+        """Opens `new_ids` as copies of a request, as it is now: they share its full pages; the page that is partly filled and
+        the fixed state are copied.  Raises `OutOfPages`, `OutOfSlots` or KeyError before anything is changed."""
+        new_ids = list(new_ids)
+        if not new_ids:
+            return
+        self._zero_new_state()
+        c = self.cache.fork(request_id, new_ids)
+        slots = list(zip(*c.slots))
+        moves = {gi: list(zip(*pairs)) for gi, pairs in c.pages.items() if pairs}
+        # every list of places in one transfer
+        lists = [l for pair in [slots] + list(moves.values()) for l in pair] + [[c.tokens] * len(new_ids)]
+        dev = iter(self._i32([x for l in lists for x in l]).split([len(l) for l in lists]))
+        src, dst = next(dev), next(dev)
+        for gi, g in enumerate(self.layout.groups):
+            if isinstance(g.need, FixedState):
+                _k.copy_pages(self.group_storage[gi], src, dst)
+        places = {gi: (next(dev), next(dev)) for gi in moves}
+        tokens = next(dev)
+        for gi, (a, b) in places.items():
+            _k.copy_pages(self.group_storage[gi], a, b, tokens if self.layout.groups[gi].need.plain else None)
+
+    def reorder(self, request_ids: Sequence[Any], parents: Sequence[int], beams: Optional[int] = None) -> None:
+        """Request r takes over what request parents[r] has computed, all at once.  Any mapping among every `beams` requests that
+        follow one another (default: all of them), which are forks of one request and of equal length."""
+        n = len(request_ids)
+        k = n if beams is None else int(beams)
+        if n == 0 and not len(parents):
+            return
+        if not 1 <= k <= _k.BEAMS_MAX or n % k or len(parents) != n or any(not 0 <= p < n or p // k != i // k for i, p in enumerate(parents)):
+            raise ValueError(f"reorder: {n} requests and the parents {list(parents)!r} in families of {k} (1 to {_k.BEAMS_MAX})")
+        if all(p == i for i, p in enumerate(parents)):
+            return
+        self._zero_new_state()
+        moves = [self.cache.reorder(request_ids[i: i + k], [p - i for p in parents[i: i + k]]) for i in range(0, n, k)]
+        paged = self.layout.paged_groups()
+        slots = [s for m in moves for s in m.slots]
+        tokens = [m.tokens for m in moves for _ in m.slots]
+        # families without a partly filled page take no part in the pages' moves: their rows lie outside
+        pages = [[p for m in moves for p in (m.pages[g] or [-1] * k)] for g in paged]
+        dev = self._i32([x for l in [list(parents), slots, tokens] + pages for x in l]).split(n)
+        for gi, g in enumerate(self.layout.groups):
+            if isinstance(g.need, FixedState):
+                _k.reorder_rows(self.group_storage[gi], dev[1], dev[0], k)
+        if any(tokens):
+            for g, rows in zip(paged, dev[3:]):
+                _k.reorder_rows(self.group_storage[g], rows, dev[0], k, dev[2] if self.layout.groups[g].need.plain else None)
+
+    def compact(self) -> int:
+        """Moves the pages that are held to the lowest numbers of their pools, on the device too; returns how many moved.  For a
+        pool whose free pages should lie together at its end, between steps."""
+        n = 0
+        for g, pairs in self.cache.compact().items():
+            if pairs:
+                src, dst = zip(*pairs)
+                dev = self._i32(src + dst)
+                _k.copy_pages(self.group_storage[g], dev[: len(src)], dev[len(src):])
+                n += len(pairs)
+        return n
+
     # --------------------------------------------------------------------------- plan
     def _validate(self, entries: Sequence[StepEntry]) -> Optional[np.ndarray]:
         """Raises `StepError` for a step that cannot be; returns the ids of a step of many tokens as one array (None: as they are)."""
@@ -415,7 +496,7 @@ class ModelRunner:
             raise StepError(f"{total} tokens exceed max_batch_tokens {self.max_batch_tokens}")
         return ids
 
-    def _build(self, entries: Sequence[StepEntry], ids: Optional[np.ndarray]) -> Tuple[StepContext, Optional[torch.Tensor]]:
+    def _build(self, entries: Sequence[StepEntry], ids: Optional[np.ndarray], beams: int = 0) -> Tuple[StepContext, Optional[torch.Tensor]]:
         ps = self.page_size
         B = len(entries)
         q_lens = np.fromiter((len(e.tokens) for e in entries), dtype=np.int64, count=B)
@@ -454,6 +535,10 @@ class ModelRunner:
             np.maximum(table, 0, out=table)
             sections += [table.reshape(-1), slot_of_token]
         sections.append(np.asarray(row_slots, dtype=np.int64))
+        shared = None
+        if beams > 1:
+            shared = np.asarray([self.cache.common_length([e.request_id for e in entries[i: i + beams]]) for i in range(0, B, beams)], dtype=np.int64)
+            sections.append(shared)
         shape = StepShape(q_lens, pos0, cu_q, kv_len, slots)
         built = [(need, need.build(shape)) for need in self.index_needs]
         for _need, arrays in built:
@@ -478,6 +563,7 @@ class ModelRunner:
             table = next(it).view(B, max_blocks)
             groups.append(GroupStep(table, next(it)))
         self.last_want_slots = next(it)
+        shared_dev = next(it) if beams > 1 else None
         indices = {need.key: tuple(next(it) for _ in arrays) for need, arrays in built}
         host_entries = [HostEntry(e.request_id, int(slots[i]), int(q_lens[i]), int(pos0[i]))
                         for i, e in enumerate(entries)]
@@ -485,12 +571,13 @@ class ModelRunner:
             num_tokens=T, num_entries=B, token_ids=views[0], positions=views[1], cu_q=views[2],
             kv_len=views[3], state_slots=views[4], groups=groups, entries=host_entries,
             max_q_len=int(q_lens.max()), max_kv_len=int(kv_len.max()), decode_only=bool((q_lens == 1).all()),
-            indices=indices)
+            indices=indices, beams=beams if beams > 1 else 0, shared_len=shared_dev,
+            max_own_len=int((kv_len[::beams] - shared).max()) if beams > 1 else 0)
         return step, (views[5] if rows else None)
 
     # --------------------------------------------------------------------------- step
     def step(self, entries: Sequence[StepEntry], device_tokens: Optional[torch.Tensor] = None,
-             borrow_logits: bool = False) -> Optional[torch.Tensor]:
+             borrow_logits: bool = False, beams: int = 0) -> Optional[torch.Tensor]:
         """Run one batch.  Returns fp32 logits [wanted, vocab] on the device in the order of
         the entries and of their `want`, or None when nothing is wanted.  Raises `OutOfPages`
         before anything runs if the cache cannot hold the new tokens (nothing is changed).
@@ -498,18 +585,23 @@ class ModelRunner:
         `device_tokens` (int32 on the device, one per entry) replaces the entries' token ids
         in a step of single tokens: the ids chosen by the last step need not visit the host
         before they are fed back.  With `borrow_logits` the result may be a view of a buffer
-        that the next step overwrites (for callers that consume it at once)."""
+        that the next step overwrites (for callers that consume it at once).
+
+        `beams` above 1: the entries are single tokens, and every `beams` of them that follow one another are forks of
+        one request (`fork`), whose common keys are read once."""
         ids = self._validate(entries)
+        if beams > 1 and (len(entries) % beams or any(len(e.tokens) != 1 for e in entries)):
+            raise StepError(f"{len(entries)} entries are no single tokens of {beams} beams a request")
         lease = self.cache.lease([(e.request_id, len(e.tokens)) for e in entries])
         try:
             self._zero_new_state()
-            bucket = self._bucket_for(entries)
+            bucket, beams = self._bucket_for(entries, beams)
             if bucket:
-                logits = self._graph_step(entries, bucket, device_tokens)
+                logits = self._graph_step(entries, bucket, device_tokens, beams)
                 if logits is not None and not borrow_logits:
                     logits = logits.clone()
             else:
-                step, rows = self._build(entries, ids)
+                step, rows = self._build(entries, ids, beams)
                 if device_tokens is not None:
                     if not step.decode_only:
                         raise StepError("device_tokens only stands for steps of single tokens")
@@ -527,22 +619,27 @@ class ModelRunner:
         return logits
 
     # ------------------------------------------------------------------ decode graphs
-    def _bucket_for(self, entries: Sequence[StepEntry]) -> int:
+    def _bucket_for(self, entries: Sequence[StepEntry], beams: int = 0) -> Tuple[int, int]:
         """Smallest captured batch size that holds a step of single tokens, else 0
-        (crates/infer-worker/src/application/runtime/graph_exec.rs:98-134)."""
+        (crates/infer-worker/src/application/runtime/graph_exec.rs:98-134), and the beams a request of that step.  Of a step of
+        beams whole requests are captured: the size is rounded to a multiple of their number, upwards where there is room."""
         if not self.use_graphs or any(len(e.tokens) != 1 for e in entries):
-            return 0
+            return 0, beams
         for c in self.capture_sizes:
             if c >= len(entries):
-                return c if c <= self.max_batch_seqs else 0
-        return 0
+                if beams > 1:
+                    up = -(-c // beams) * beams
+                    return (up if up <= self.max_batch_seqs else c // beams * beams), beams
+                return (c if c <= self.max_batch_seqs else 0), beams
+        return 0, beams
 
     def _graph_step(self, entries: Sequence[StepEntry], bucket: int,
-                    device_tokens: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-        g = self._graphs.get(bucket)
+                    device_tokens: Optional[torch.Tensor], beams: int = 0) -> Optional[torch.Tensor]:
+        key = (bucket, beams) if beams > 1 else bucket
+        g = self._graphs.get(key)
         if g is None:
-            g = _DecodeGraph(self, bucket)
-            self._graphs[bucket] = g
+            g = _DecodeGraph(self, bucket, beams)
+            self._graphs[key] = g
         g.fill(self, entries, device_tokens is None)
         if device_tokens is not None:
             g.step.token_ids[: len(entries)].copy_(device_tokens[: len(entries)])
@@ -566,7 +663,6 @@ class ModelRunner:
         """Raise if a kernel recorded a fault it survived (a bounded wait that ran out).
         Reads one word from the device, so it synchronises; callers use it where they
         synchronise anyway."""
-        from ..ops import kernels as _k
         code = _k.gemm_tc_error(self.device)
         if code:
             what = ("its shared memory did not start on a 1024-byte boundary" if code == 14

@@ -2145,14 +2145,15 @@ def attention_beams_supports(num_heads: int, num_kv_heads: int, head_dim: int) -
 @functools.lru_cache(maxsize=4096)
 def attention_beams_splits(rows: int, beams: int, num_heads: int, num_kv_heads: int, head_dim: int, most_shared: int, most_own: int,
                            num_sms: int) -> Tuple[int, int]:
-    """Ranges that the shared keys of a group, and the keys of a row's own, are cut into: about a wave of CTAs for the former."""
+    """Ranges that the shared keys of a group, and the keys of a row's own, are cut into (16 at most in all, for scratch that is made for
+    `GQAAttention.MAX_SPLITS`): about a wave of CTAs for the former."""
     lib = L.attention_beams(head_dim)
     group = num_heads // num_kv_heads
     row_tiles = int(lib.ri_attention_beams_row_tiles(beams * group))
     slots = int(lib.ri_attention_beams_ctas_per_sm(row_tiles)) * num_sms
     ctas = rows // beams * num_kv_heads * -(-beams * group // (16 * row_tiles))
-    shared = max(1, min(slots // max(1, ctas), -(-most_shared // 128), 16))
-    return shared, max(1, min(-(-most_own // 256), 8))
+    shared = max(1, min(slots // max(1, ctas), -(-most_shared // 128), 12))
+    return shared, max(1, min(-(-most_own // 256), 4))
 
 
 def attention_decode_beams(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,

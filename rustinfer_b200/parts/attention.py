@@ -266,7 +266,7 @@ class GQAAttention(Mixer):
         """Key ranges a step of single tokens only is cut into when its caller merges them itself
         (`attend(..., merge=False)`); 0 when there is nothing to merge (another kind of step, one
         range, or the kernel without ranges)."""
-        if not self.use_mma or not step.decode_only:
+        if not self.use_mma or not step.decode_only or step.beams > 1:
             return 0
         splits = self._splits(step.num_tokens, step.max_kv_len)
         return splits if splits > 1 else 0
@@ -305,6 +305,10 @@ class GQAAttention(Mixer):
             tile_entry, tile_q0 = step.index(self._tiles)
             K.attention_plain(q, out, cache.kv, g.block_table, step.cu_q, step.kv_len, tile_entry, tile_q0,
                               self.Hq, self.Hkv, self.hd, self.scale, self.window, self.block, self.vd, sink=self.sink)
+            return out
+        if step.beams > 1:                            # the keys the beams of a request share are read once for all of them
+            K.attention_decode_beams(q, out, cache.kv, g.block_table, step.kv_len, step.shared_len, step.beams, self.Hq, self.Hkv, self.hd,
+                                     self.scale, self.window, step.max_kv_len, step.max_own_len, self.part_o, self.part_lse)
             return out
         (single,) = step.index(self._single)
         if single.numel():
