@@ -5,14 +5,20 @@
 //
 // Keys before shared_len[g] are the same for every row of group g, whose rows follow one another: one CTA reads a range of them, by the
 // first row's table, for all beams x heads of a key head, which are the M dimension of the matrix products.  Keys from there on are read
-// by each row's own table.  Both leave partial results (a sum weighted by 2^(score - maximum), its log-sum-exp in base 2) that a second
-// kernel joins.  RustInfer's decode attention reads a request's keys for that request alone
+// by each row's own table, by a warp for one key head's heads.  Both leave partial results (a sum weighted by 2^(score - maximum), its
+// log-sum-exp in base 2) that a second kernel joins.  RustInfer's decode attention reads a request's keys for that request alone
 // (crates/infer-backend-cuda/src/kernels/flash_attn_gqa/flash_attn_paged_decode.cu:75-340).
 //
 // What bounds it is the cache's stream: shared keys and values once a request, the beams' own once a beam.  Scores, maxima, sums and
 // outputs are 32-bit.  A weight enters the product with the values as two bf16 pieces that add up to it to 2^-17 of itself: rounded to one
 // piece it would be off by up to 2^-9, as much as the stored output's own rounding.
+//
+// Shared keys come by TMA where the head size is 64 or 128 and a page holds 8, 16, 32 or a multiple of 64 keys (a box a page and 64 columns,
+// each from a lane of its own; the 128-byte swizzle, which ldmatrix reads through), else by cp.async: half of the loop's instructions were
+// the latter's addresses.
 #include "common.cuh"
+#include <cuda.h>
+#include <mutex>
 
 #ifndef RI_HEAD_DIM
 #error "compile with -DRI_HEAD_DIM=<head size>"
@@ -21,15 +27,25 @@
 namespace {
 constexpr int HD = RI_HEAD_DIM;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "beam attention: head size multiple of 16, at most 256");
-constexpr int KT = 64;                                     // keys a tile
 constexpr int ROW = HD + 8;                                // padded rows: 16 bytes on, ldmatrix meets no bank twice
+constexpr int OROW = HD + 8;                               // rows of outputs in shared memory: pairs of lanes apart
 constexpr int CH = HD / 8;                                 // 16-byte pieces a row
 constexpr int KS = HD / 16;
 constexpr int NT = HD / 8;
-constexpr int WARPS = 4;
+constexpr int WARPS = 8;
 constexpr int THREADS = 32 * WARPS;
-constexpr int STAGES = HD <= 128 ? 3 : 2;
+constexpr int CTAS = HD <= 128 ? 2 : 1;                    // CTAs an SM that registers and shared memory are cut for
 constexpr int MAX_BEAMS = 64;
+constexpr int OWN_KEYS = 16;                               // keys of its own a row's warp takes at a time
+constexpr bool BY_TMA = HD == 64 || HD == 128;
+constexpr int TKB = HD / 64;                               // 64-column blocks of a head
+constexpr unsigned SPIN_LIMIT = 1u << 20;
+
+// Keys of a tile: 32 a warp where a CTA has room for two or three of them
+template <int RTILES> constexpr int tile_keys() { return HD <= 64 && RTILES <= 2 ? 128 : 64; }
+constexpr int STAGES = HD <= 64 ? 3 : 2;
+// rows of shared keys are split over RTILES warps, a tile's keys over the others
+template <int RTILES> constexpr int key_groups() { return WARPS / RTILES < tile_keys<RTILES>() / 16 ? WARPS / RTILES : tile_keys<RTILES>() / 16; }
 
 __device__ __forceinline__ void cp_async16(void* smem, const void* gmem, bool valid) {
     const unsigned s = (unsigned)__cvta_generic_to_shared(smem);
@@ -52,6 +68,43 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const unsigned (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ float ex2(float x) {            // 2 ulp
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint64_t* bar) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t* bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+// bounded: false after SPIN_LIMIT tries
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, unsigned parity) {
+#pragma unroll 1
+    for (unsigned i = 0; i < SPIN_LIMIT; ++i) {
+        unsigned ok;
+        asm volatile("{\n\t.reg .pred p;\n\t"
+                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                     "selp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+        if (ok) return true;
+        if (i > 1024) __nanosleep(64);
+    }
+    return false;
+}
+__device__ __forceinline__ void tma_load_2d(void* smem, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(smem_u32(smem)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
+}
+// d (8 rows x 8 columns of a 16 x 8 product whose lower rows are zero) += a b
+__device__ __forceinline__ void mma_8rows(float (&d)[2], unsigned a0, unsigned a2, unsigned b0, unsigned b1) {
+    [[maybe_unused]] float x, y;
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "=f"(x), "=f"(y)
+                 : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
+}
 // two weights as bf16 pairs: the rounded weights, and what the rounding left
 __device__ __forceinline__ void two_pieces(float a, float b, unsigned& high, unsigned& low) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
@@ -70,9 +123,11 @@ struct Args {
     const int* shared_len;
     int beams, Hq, Hkv, page_size;
     float scale_log2;
-    int window, shared_splits, own_splits;
+    int window, groups, shared_splits, own_splits, target;
     float* part_o;
     float* part_lse;
+    int* error;
+    int box_rows;                                          // rows of a TMA box: a page's, or a tile's of a large one
 };
 
 // A row's keys: no more than its table has pages for, whatever it is said to have
@@ -95,18 +150,107 @@ __device__ __forceinline__ void shared_range(const Args& a, int g, int& from, in
     to = same && s > lo ? s : lo;
 }
 
-// Keys [lo, hi) by table row `bt` for the rows m0 .. m0 + m_count - 1 (of beams x heads) of group g, RTILES tiles of 16 rows in one CTA.
-template <int RTILES>
-__device__ __forceinline__ void attend(const Args& a, unsigned char* smem, int g, int kvh, int m0, int m_count, const int* bt, int lo, int hi, int part) {
-    constexpr int KG = WARPS / RTILES;                     // warps that share a row tile take parts of a tile's keys
+// Keys [lo, hi) by table row `bt` for the rows m0 .. m0 + m_count - 1 (of beams x heads) of group g, RTILES tiles of 16 rows in one CTA.  Tiles
+// lie where the multiples of their size do, so that a page's keys lie in one.
+template <int RTILES, bool TMA>
+__device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, unsigned char* smem, int g, int kvh, int m0, int m_count, const int* bt,
+                                       int lo, int hi, int part) {
+    constexpr int KT = tile_keys<RTILES>(), KG = key_groups<RTILES>();
     constexpr int WK = KT / KG;                            // keys a warp takes of a tile
     constexpr int NK = WK / 8;
+    constexpr int PIECES = (KT * CH + THREADS - 1) / THREADS;      // 16-byte pieces of a tile's keys a thread fetches
+    constexpr int KROW = TMA ? HD : ROW;
+    constexpr int STAGE = 2 * KT * KROW;                   // elements
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.Hq / a.Hkv, splits = a.shared_splits + a.own_splits;
-    bf16* Qs = reinterpret_cast<bf16*>(smem);              // [RTILES * 16][ROW]
-    bf16* KVs = Qs + RTILES * 16 * ROW;                    // [STAGES][K | V][KT][ROW]
+    bf16* KVs = reinterpret_cast<bf16*>(smem);             // [STAGES][K | V][KT][KROW]
+    bf16* Qs = KVs + STAGES * STAGE;                       // [RTILES * 16][ROW]
+    uint64_t* full = reinterpret_cast<uint64_t*>(Qs + RTILES * 16 * ROW);
     const int rt = warp / KG, kg = warp % KG;
+    const bool works = warp < RTILES * KG;
 
+    const int t0 = lo / KT, tiles = (hi + KT - 1) / KT - t0;
+    const size_t head_step = (size_t)a.page_size * HD, value_step = (size_t)a.Hkv * head_step;
+    const int shift = (a.page_size & (a.page_size - 1)) == 0 ? __ffs(a.page_size) - 1 : -1;
+    // cp.async: where a thread's pieces of a tile lie, looked up a tile ahead of the fetch
+    const bf16* from[PIECES];
+    auto look_up = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int c = tid + i * THREADS, kk = c / CH, ch = c - kk * CH, key = (t0 + t) * KT + kk;
+            from[i] = nullptr;
+            if (c < KT * CH && key >= lo && key < hi) {
+                const int blk = shift >= 0 ? key >> shift : key / a.page_size;
+                from[i] = a.cache + ((size_t)bt[blk] * 2 * a.Hkv + kvh) * head_step + (size_t)(key - blk * a.page_size) * HD + ch * 8;
+            }
+        }
+    };
+    // TMA, the first warp: a lane's box is keys or values, a page of the tile, 64 columns; its page's number is read a tile ahead
+    const int boxes = KT / a.box_rows;                     // of keys, of 64 columns
+    constexpr int MOST_BOXES = 2 * (KT / 8) * (BY_TMA ? TKB : 1);
+    constexpr int TURNS = (MOST_BOXES + 31) / 32;          // (pages of 8 keys: more boxes than lanes)
+    int row_of[TURNS];
+    auto look_up_boxes = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+            const int box = lane + 32 * i, kv = box / (boxes * TKB), c = (box - kv * boxes * TKB) / TKB, key = (t0 + t) * KT + c * a.box_rows;
+            row_of[i] = -1;                                // boxes without a key in [lo, hi) are not fetched
+            if (box < 2 * boxes * TKB && key < hi && key + a.box_rows > lo) {
+                const int blk = key / a.page_size;
+                row_of[i] = ((bt[blk] * 2 + kv) * a.Hkv + kvh) * a.page_size + (key - blk * a.page_size);
+            }
+        }
+    };
+    auto fetch = [&](int t, int stage) {                   // tile t, which was looked up; looks up the next
+        if constexpr (TMA) {
+            if (warp == 0) {
+                int mine = 0;
+#pragma unroll
+                for (int i = 0; i < TURNS; ++i) mine += row_of[i] >= 0;
+                const int all = __reduce_add_sync(0xffffffffu, mine);
+                if (lane == 0) bar_expect(&full[stage], (unsigned)all * a.box_rows * 128);
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < TURNS; ++i) {
+                    const int box = lane + 32 * i, kv = box / (boxes * TKB), rest = box - kv * boxes * TKB, c = rest / TKB, kb = rest - c * TKB;
+                    if (row_of[i] >= 0)
+                        tma_load_2d(reinterpret_cast<unsigned char*>(KVs + stage * STAGE) + ((kv * TKB + kb) * KT + c * a.box_rows) * 128, map,
+                                    &full[stage], kb * 64, row_of[i]);
+                }
+                if (t + 1 < tiles) look_up_boxes(t + 1);
+            }
+        } else {
+            bf16* Ks = KVs + stage * STAGE;
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int c = tid + i * THREADS, kk = c / CH, ch = c - kk * CH;
+                if (c < KT * CH) {
+                    const bool ok = from[i] != nullptr;
+                    const bf16* k = ok ? from[i] : a.cache;
+                    cp_async16(Ks + kk * ROW + ch * 8, k, ok);
+                    cp_async16(Ks + (KT + kk) * ROW + ch * 8, ok ? k + value_step : k, ok);
+                }
+            }
+            if (t + 1 < tiles) look_up(t + 1);
+        }
+    };
+    if constexpr (TMA) {
+        if (tid == 0) {
+            for (int s = 0; s < STAGES; ++s) bar_init(&full[s]);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        if (warp == 0) {
+            look_up_boxes(0);
+            __syncwarp();
+        }
+    } else {
+        look_up(0);
+    }
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) {
+        if (s < tiles) fetch(s, s);
+        if constexpr (!TMA) cp_async_commit();
+    }
     for (int c = tid; c < RTILES * 16 * CH; c += THREADS) {
         const int r = c / CH, ch = c - r * CH, m = m0 + r;
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
@@ -116,91 +260,105 @@ __device__ __forceinline__ void attend(const Args& a, unsigned char* smem, int g
         }
         *reinterpret_cast<uint4*>(Qs + r * ROW + ch * 8) = v;
     }
-    const size_t head_step = (size_t)a.page_size * HD;
-    const int shift = (a.page_size & (a.page_size - 1)) == 0 ? __ffs(a.page_size) - 1 : -1;
-    auto load = [&](int k0, int stage) {
-        bf16* Ks = KVs + (size_t)stage * 2 * KT * ROW;
-        bf16* Vs = Ks + KT * ROW;
-        for (int c = tid; c < KT * CH; c += THREADS) {
-            const int kk = c / CH, ch = c - kk * CH, key = k0 + kk;
-            const bool ok = key < hi;
-            const bf16 *sk = a.cache, *sv = a.cache;
-            if (ok) {
-                const int blk = shift >= 0 ? key >> shift : key / a.page_size;
-                const int off = key - blk * a.page_size;
-                sk = a.cache + ((size_t)bt[blk] * 2 * a.Hkv + kvh) * head_step + (size_t)off * HD + ch * 8;
-                sv = sk + (size_t)a.Hkv * head_step;
-            }
-            cp_async16(Ks + kk * ROW + ch * 8, sk, ok);
-            cp_async16(Vs + kk * ROW + ch * 8, sv, ok);
-        }
-    };
-    const int tiles = hi > lo ? (hi - lo + KT - 1) / KT : 0;
-#pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) {
-        if (s < tiles) load(lo + s * KT, s);
-        cp_async_commit();
-    }
-    __syncthreads();
-    unsigned qf[KS][4];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) ldmatrix_x4(qf[ks], Qs + (rt * 16 + (lane & 15)) * ROW + ks * 16 + (lane >> 4) * 8);
     float o[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    __syncthreads();                                       // queries are there, and the barriers
 
-    for (int t = 0; t < tiles; ++t) {
-        cp_async_wait<STAGES - 2>();
-        __syncthreads();                                   // the tile has come, and the one before it is used up
-        if (t + STAGES - 1 < tiles) load(lo + (t + STAGES - 1) * KT, (t + STAGES - 1) % STAGES);
-        cp_async_commit();
-        const bf16* Ks = KVs + (size_t)(t % STAGES) * 2 * KT * ROW;
-        const bf16* Vs = Ks + KT * ROW;
-        const int kw0 = kg * WK, key0 = lo + t * KT + kw0;
-        if (key0 >= hi) continue;
+    unsigned parity = 0;
+    for (int t = 0, stage = 0; t < tiles; ++t) {
+        // the tile has come, and the one before it is used up
+        if constexpr (TMA) {
+            if (!__syncthreads_and(bar_wait(&full[stage], parity))) {
+                // a wait ran out: the copies behind are waited for too, with the same limit, and the host is told
+                for (int u = t; u < min(tiles, t + STAGES - 1); ++u) {
+                    bar_wait(&full[stage], parity);
+                    if (++stage == STAGES) { stage = 0; parity ^= 1u; }
+                }
+                if (tid == 0) atomicExch(a.error, 22);
+                break;
+            }
+        } else {
+            cp_async_wait<STAGES - 2>();
+            __syncthreads();
+        }
+        if (t + STAGES - 1 < tiles) fetch(t + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+        if constexpr (!TMA) cp_async_commit();
+        bf16* Ks = KVs + stage * STAGE;
+        bf16* Vs = Ks + KT * KROW;
+        if (++stage == STAGES) { stage = 0; parity ^= 1u; }
+        const int kw0 = kg * WK, key0 = (t0 + t) * KT + kw0;
+        if (!works || key0 >= hi || key0 + WK <= lo) continue;
+        const bool edge = key0 < lo || key0 + WK > hi;
+        // where the 16 bytes of columns col .. col + 7 of row `row` lie
+        auto at = [&](bf16* tile, int row, int col) -> bf16* {
+            if constexpr (TMA) return tile + (col >> 6) * (KT * 64) + row * 64 + ((((col & 63) >> 3) ^ (row & 7)) << 3);
+            else return tile + row * ROW + col;
+        };
+        if constexpr (TMA) {
+            if (edge) {
+                // values of keys outside meet a weight of zero, but what lies there may be no number
+                for (int i = lane; i < WK * CH; i += 32) {
+                    const int r = i / CH, key = key0 + r;
+                    if (key < lo || key >= hi) *reinterpret_cast<uint4*>(at(Vs, kw0 + r, (i - r * CH) * 8)) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // ahead of the copy that the stage is used for next
+                __syncwarp();
+            }
+        }
         float s[NK][4];
 #pragma unroll
         for (int n = 0; n < NK; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+        for (int ks = 0; ks < KS; ++ks) {
+            unsigned qf[4];                                // (from shared memory every tile: its registers make room for a second CTA)
+            ldmatrix_x4(qf, Qs + (rt * 16 + (lane & 15)) * ROW + ks * 16 + (lane >> 4) * 8);
 #pragma unroll
             for (int n2 = 0; n2 < NK / 2; ++n2) {
                 unsigned kf[4];
-                ldmatrix_x4(kf, Ks + (kw0 + n2 * 16 + (lane & 7) + (lane >> 4) * 8) * ROW + ks * 16 + ((lane >> 3) & 1) * 8);
-                mma_bf16(s[2 * n2], qf[ks], kf[0], kf[1]);
-                mma_bf16(s[2 * n2 + 1], qf[ks], kf[2], kf[3]);
+                ldmatrix_x4(kf, at(Ks, kw0 + n2 * 16 + (lane & 7) + (lane >> 4) * 8, ks * 16 + ((lane >> 3) & 1) * 8));
+                mma_bf16(s[2 * n2], qf, kf[0], kf[1]);
+                mma_bf16(s[2 * n2 + 1], qf, kf[2], kf[3]);
             }
+        }
         float mx[2] = {-INFINITY, -INFINITY};
-        const int left = hi - key0;                        // keys of this warp's that exist
+        if (edge) {
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int key = key0 + n * 8 + (lane & 3) * 2 + (e & 1);
+                    if (key < lo || key >= hi) s[n][e] = -INFINITY;
+                }
+        }
 #pragma unroll
         for (int n = 0; n < NK; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[n][e] = n * 8 + (lane & 3) * 2 + (e & 1) < left ? s[n][e] * a.scale_log2 : -INFINITY;
-                mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
-            }
+            for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
         float alpha[2], muse[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2)) * a.scale_log2;
             const float mnew = fmaxf(m[i], mx[i]);
             muse[i] = mnew == -INFINITY ? 0.f : mnew;
-            alpha[i] = exp2f(m[i] - muse[i]);
+            alpha[i] = ex2(m[i] - muse[i]);
             m[i] = mnew;
             l[i] *= alpha[i];
         }
+        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            o[n][0] *= alpha[0]; o[n][1] *= alpha[0];
-            o[n][2] *= alpha[1]; o[n][3] *= alpha[1];
+            for (int n = 0; n < NT; ++n) {
+                o[n][0] *= alpha[0]; o[n][1] *= alpha[0];
+                o[n][2] *= alpha[1]; o[n][3] *= alpha[1];
+            }
         }
 #pragma unroll
         for (int n = 0; n < NK; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                s[n][e] = exp2f(s[n][e] - muse[e >> 1]);
+                s[n][e] = ex2(fmaf(s[n][e], a.scale_log2, -muse[e >> 1]));
                 l[e >> 1] += s[n][e];
             }
 #pragma unroll
@@ -213,7 +371,7 @@ __device__ __forceinline__ void attend(const Args& a, unsigned char* smem, int g
 #pragma unroll
             for (int np = 0; np < NT / 2; ++np) {
                 unsigned vf[4];
-                ldmatrix_x4_trans(vf, Vs + (kw0 + n2 * 16 + (lane & 15)) * ROW + np * 16 + (lane >> 4) * 8);
+                ldmatrix_x4_trans(vf, at(Vs, kw0 + n2 * 16 + (lane & 15), np * 16 + (lane >> 4) * 8));
                 mma_bf16(o[2 * np], ph, vf[0], vf[1]);
                 mma_bf16(o[2 * np + 1], ph, vf[2], vf[3]);
                 mma_bf16(o[2 * np], pl, vf[0], vf[1]);
@@ -221,139 +379,361 @@ __device__ __forceinline__ void attend(const Args& a, unsigned char* smem, int g
             }
         }
     }
-    cp_async_wait<0>();
+    if constexpr (!TMA) cp_async_wait<0>();
     __syncthreads();
 
     // the warps' states through shared memory (the tiles are used up)
-    float* Os = reinterpret_cast<float*>(KVs);             // [WARPS][16][HD]
-    float* Ms = Os + WARPS * 16 * HD;                      // [WARPS][16]
+    float* Os = reinterpret_cast<float*>(KVs);             // [WARPS][16][OROW]
+    float* Ms = Os + WARPS * 16 * OROW;                    // [WARPS][16]
     float* Ls = Ms + WARPS * 16;
+    if (works)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        const int r = (lane >> 2) + 8 * i;
-        float* orow = Os + ((size_t)warp * 16 + r) * HD + (lane & 3) * 2;
+        for (int i = 0; i < 2; ++i) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+            const int r = (lane >> 2) + 8 * i;
+            float* orow = Os + (warp * 16 + r) * OROW + (lane & 3) * 2;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(orow + n * 8) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
-        if ((lane & 3) == 0) { Ms[warp * 16 + r] = m[i]; Ls[warp * 16 + r] = l[i]; }
-    }
+            for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(orow + n * 8) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+            if ((lane & 3) == 0) { Ms[warp * 16 + r] = m[i]; Ls[warp * 16 + r] = l[i]; }
+        }
     __syncthreads();
-    for (int idx = tid; idx < m_count * HD; idx += THREADS) {
-        const int r = idx / HD, d = idx - r * HD, w0 = (r >> 4) * KG, rr = r & 15;
+    for (int r = warp; r < m_count; r += WARPS) {          // a warp a row
+        const int w0 = (r >> 4) * KG, rr = r & 15;
         float M = -INFINITY;
 #pragma unroll
         for (int w = 0; w < KG; ++w) M = fmaxf(M, Ms[(w0 + w) * 16 + rr]);
-        float L = 0.f, O = 0.f;
         const float muse = M == -INFINITY ? 0.f : M;
+        float f[KG], L = 0.f;
 #pragma unroll
         for (int w = 0; w < KG; ++w) {
-            const float f = exp2f(Ms[(w0 + w) * 16 + rr] - muse);
-            L += Ls[(w0 + w) * 16 + rr] == 0.f ? 0.f : Ls[(w0 + w) * 16 + rr] * f;
-            O += Ls[(w0 + w) * 16 + rr] == 0.f ? 0.f : Os[((size_t)(w0 + w) * 16 + rr) * HD + d] * f;
+            const float lw = Ls[(w0 + w) * 16 + rr];
+            f[w] = lw == 0.f ? 0.f : ex2(Ms[(w0 + w) * 16 + rr] - muse);
+            L += lw * f[w];
         }
+        const float inv = L == 0.f ? 0.f : 1.f / L;
         const int mm = m0 + r, b = mm / G, h = mm - b * G;
         const size_t p = ((size_t)(g * a.beams + b) * a.Hq + kvh * G + h) * splits + part;
-        a.part_o[p * HD + d] = L == 0.f ? 0.f : O / L;
-        if (d == 0) a.part_lse[p] = L == 0.f ? -INFINITY : muse + log2f(L);      // what is no number stays none
+        for (int d = lane * 4; d < HD; d += 128) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < KG; ++w) {
+                const float4 x = *reinterpret_cast<const float4*>(Os + ((w0 + w) * 16 + rr) * OROW + d);
+                if (f[w] != 0.f) { v.x += x.x * f[w]; v.y += x.y * f[w]; v.z += x.z * f[w]; v.w += x.w * f[w]; }
+            }
+            *reinterpret_cast<float4*>(a.part_o + p * HD + d) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        }
+        if (lane == 0) a.part_lse[p] = L == 0.f ? -INFINITY : muse + log2f(L);               // what is no number stays none
     }
 }
 
-// Blocks: first (group, key head, row chunk, range of shared keys), then (row, key head, head chunk, range of the row's own keys).
-template <int RTILES>
-__global__ void __launch_bounds__(THREADS)
-beams_kernel(Args a, int groups, int chunks, int own_chunks) {
-    extern __shared__ __align__(16) unsigned char smem[];
-    pdl_wait();
-    pdl_trigger();
-    const int G = a.Hq / a.Hkv;
-    int id = blockIdx.x, from, to;
-    const int n_shared = groups * a.Hkv * chunks * a.shared_splits;
-    if (id < n_shared) {
-        const int split = id % a.shared_splits;  id /= a.shared_splits;
-        const int chunk = id % chunks;           id /= chunks;
-        const int kvh = id % a.Hkv, g = id / a.Hkv;
-        shared_range(a, g, from, to);
-        const int tiles = (to - from + KT - 1) / KT, per = (tiles + a.shared_splits - 1) / a.shared_splits;
-        const int lo = min(to, from + split * per * KT), hi = min(to, lo + per * KT);
-        const int m0 = chunk * RTILES * 16;
-        attend<RTILES>(a, smem, g, kvh, m0, min(RTILES * 16, a.beams * G - m0), a.table + (size_t)g * a.beams * a.table_stride, lo, hi, split);
+// A row's own keys [lo, hi) for up to 8 heads of one key head, by one warp: 16 keys at a time, the next keys on their way while the values are
+// used and the other way round.
+__device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, int r, int kvh, int head0, int heads, int lo, int hi, int part) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int splits = a.shared_splits + a.own_splits;
+    bf16* Ks = reinterpret_cast<bf16*>(smem) + warp * 2 * OWN_KEYS * ROW;
+    bf16* Vs = Ks + OWN_KEYS * ROW;
+    const int* bt = a.table + (size_t)r * a.table_stride;
+    const size_t head_step = (size_t)a.page_size * HD, value_step = (size_t)a.Hkv * head_step;
+    auto fetch = [&](bf16* to, int k0, size_t step) {      // a lane a row's half: 16 rows, two lanes each
+        const int kk = lane >> 1, key = k0 + kk;
+        const bool there = key < hi;
+        const bf16* src = a.cache;
+        if (there) {
+            const int blk = key / a.page_size;
+            src = a.cache + ((size_t)bt[blk] * 2 * a.Hkv + kvh) * head_step + (size_t)(key - blk * a.page_size) * HD + step;
+        }
+#pragma unroll
+        for (int ch = 0; ch < CH / 2; ++ch) {
+            const int c = 2 * ch + (lane & 1);
+            cp_async16(to + kk * ROW + c * 8, there ? src + c * 8 : src, there);
+        }
+        cp_async_commit();
+    };
+    const size_t p0 = ((size_t)r * a.Hq + head0) * splits + part;       // of the first head; the next is `splits` on
+    if (lo >= hi) {
+        if (lane < heads) a.part_lse[p0 + (size_t)lane * splits] = -INFINITY;
         return;
     }
-    id -= n_shared;
-    const int split = id % a.own_splits;  id /= a.own_splits;
+    fetch(Ks, lo, 0);
+    fetch(Vs, lo, value_step);
+    unsigned qf[KS][2];                                    // rows 0 to 7 alone
+    {
+        const int h = lane >> 2;
+        const bf16* q = a.q + (size_t)r * a.q_stride + (size_t)(head0 + h) * HD + (lane & 3) * 2;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            qf[ks][0] = h < heads ? *reinterpret_cast<const unsigned*>(q + ks * 16) : 0u;
+            qf[ks][1] = h < heads ? *reinterpret_cast<const unsigned*>(q + ks * 16 + 8) : 0u;
+        }
+    }
+    float o[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    for (int k0 = lo; k0 < hi; k0 += OWN_KEYS) {
+        cp_async_wait<1>();
+        __syncwarp();
+        float s[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            unsigned kf[4];
+            ldmatrix_x4(kf, Ks + ((lane & 7) + (lane >> 4) * 8) * ROW + ks * 16 + ((lane >> 3) & 1) * 8);
+            mma_8rows(s[0], qf[ks][0], qf[ks][1], kf[0], kf[1]);
+            mma_8rows(s[1], qf[ks][0], qf[ks][1], kf[2], kf[3]);
+        }
+        __syncwarp();
+        if (k0 + OWN_KEYS < hi) fetch(Ks, k0 + OWN_KEYS, 0);
+        else cp_async_commit();
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (k0 + n * 8 + (lane & 3) * 2 + e >= hi) s[n][e] = -INFINITY;
+                mx = fmaxf(mx, s[n][e]);
+            }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * a.scale_log2;
+        const float mnew = fmaxf(m, mx), muse = mnew == -INFINITY ? 0.f : mnew, alpha = ex2(m - muse);
+        m = mnew;
+        l *= alpha;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) { o[n][0] *= alpha; o[n][1] *= alpha; }
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                s[n][e] = ex2(fmaf(s[n][e], a.scale_log2, -muse));
+                l += s[n][e];
+            }
+        unsigned ph[2], pl[2];
+        two_pieces(s[0][0], s[0][1], ph[0], pl[0]);
+        two_pieces(s[1][0], s[1][1], ph[1], pl[1]);
+        cp_async_wait<1>();
+        __syncwarp();
+#pragma unroll
+        for (int np = 0; np < NT / 2; ++np) {
+            unsigned vf[4];
+            ldmatrix_x4_trans(vf, Vs + (lane & 15) * ROW + np * 16 + (lane >> 4) * 8);
+            mma_8rows(o[2 * np], ph[0], ph[1], vf[0], vf[1]);
+            mma_8rows(o[2 * np + 1], ph[0], ph[1], vf[2], vf[3]);
+            mma_8rows(o[2 * np], pl[0], pl[1], vf[0], vf[1]);
+            mma_8rows(o[2 * np + 1], pl[0], pl[1], vf[2], vf[3]);
+        }
+        __syncwarp();
+        if (k0 + OWN_KEYS < hi) fetch(Vs, k0 + OWN_KEYS, value_step);
+        else cp_async_commit();
+    }
+    cp_async_wait<0>();
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    const int h = lane >> 2;
+    if (h < heads) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const size_t p = p0 + (size_t)h * splits;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+            *reinterpret_cast<float2*>(a.part_o + p * HD + n * 8 + (lane & 3) * 2) = make_float2(o[n][0] * inv, o[n][1] * inv);
+        if ((lane & 3) == 0) a.part_lse[p] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
+    }
+}
+
+// Tiles of shared keys a CTA takes: as many as make about `target` CTAs of all groups' tiles together, and no more ranges of the longest
+// than there is room for
+__device__ __forceinline__ int tiles_a_range(const Args& a, int ctas_a_range, int KT) {
+    const int lane = threadIdx.x & 31;
+    int total = 0, most = 0;
+    for (int g = lane; g < a.groups; g += 32) {
+        const int n = keys_of(a, g * a.beams), lo = a.window > 0 ? max(0, n - a.window) : 0, hi = max(lo, min(a.shared_len[g], n));
+        const int tiles = (hi + KT - 1) / KT - lo / KT;
+        total += tiles;
+        most = max(most, tiles);
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    most = __reduce_max_sync(0xffffffffu, most);
+    return max(1, max((int)(((long long)total * ctas_a_range + a.target - 1) / a.target), (most + a.shared_splits - 1) / a.shared_splits));
+}
+
+// Blocks: first (range of shared keys, group, key head, row chunk), then a warp for (range of the row's own keys, row, key head, eight heads).
+template <int RTILES, bool TMA>
+__global__ void __launch_bounds__(THREADS, CTAS)
+beams_kernel(const __grid_constant__ CUtensorMap map, Args a, int chunks, int own_chunks) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    pdl_wait();
+    pdl_trigger();
+    constexpr int KT = tile_keys<RTILES>();
+    const int G = a.Hq / a.Hkv;
+    int id = blockIdx.x, from, to;
+    const int n_shared = a.groups * a.Hkv * chunks * a.shared_splits;
+    if (id < n_shared) {
+        const int chunk = id % chunks;        id /= chunks;
+        const int kvh = id % a.Hkv;           id /= a.Hkv;
+        const int g = id % a.groups, split = id / a.groups;
+        shared_range(a, g, from, to);
+        const int per = tiles_a_range(a, a.Hkv * chunks, KT);
+        // ranges start at multiples of the tiles' size
+        const int lo = split == 0 ? from : (int)min((long long)to, ((long long)(from / KT) + (long long)split * per) * KT);
+        const int hi = (int)min((long long)to, ((long long)(from / KT) + (long long)(split + 1) * per) * KT);
+        const int m0 = chunk * RTILES * 16, m_count = min(RTILES * 16, a.beams * G - m0);
+        if (lo >= hi) {                                    // the range is empty: that is all there is to say
+            for (int r = threadIdx.x; r < m_count; r += THREADS) {
+                const int b = (m0 + r) / G, h = m0 + r - b * G;
+                a.part_lse[((size_t)(g * a.beams + b) * a.Hq + kvh * G + h) * (a.shared_splits + a.own_splits) + split] = -INFINITY;
+            }
+            return;
+        }
+        attend<RTILES, TMA>(a, &map, smem, g, kvh, m0, m_count, a.table + (size_t)g * a.beams * a.table_stride, lo, hi, split);
+        return;
+    }
+    id = (id - n_shared) * WARPS + (threadIdx.x >> 5);
     const int chunk = id % own_chunks;    id /= own_chunks;
-    const int kvh = id % a.Hkv, r = id / a.Hkv, g = r / a.beams, b = r - g * a.beams;
-    shared_range(a, g, from, to);
+    const int kvh = id % a.Hkv;           id /= a.Hkv;
+    const int split = id % a.own_splits, r = id / a.own_splits;
+    if (r >= a.groups * a.beams) return;
+    shared_range(a, r / a.beams, from, to);
     const int end = keys_of(a, r);
     const int begin = to > from ? to : (a.window > 0 ? max(0, end - a.window) : 0);
-    const int tiles = (max(0, end - begin) + KT - 1) / KT, per = (tiles + a.own_splits - 1) / a.own_splits;
-    const int lo = min(end, begin + split * per * KT), hi = min(end, lo + per * KT);
-    attend<1>(a, smem, g, kvh, b * G + chunk * 16, min(16, G - chunk * 16), a.table + (size_t)r * a.table_stride, lo, hi, a.shared_splits + split);
+    const int steps = (max(0, end - begin) + OWN_KEYS - 1) / OWN_KEYS, per = (steps + a.own_splits - 1) / a.own_splits;
+    const int lo = (int)min((long long)end, begin + (long long)split * per * OWN_KEYS), hi = min(end, lo + per * OWN_KEYS);
+    attend_own(a, smem, r, kvh, kvh * G + chunk * 8, min(8, G - chunk * 8), lo, hi, a.shared_splits + split);
 }
 
-// out[r, h, :] = sum over ranges of 2^(lse - max) part / sum of 2^(lse - max); a row without keys: zeros
-__global__ void beams_join_kernel(const float* part_o, const float* part_lse, bf16* out, int out_stride, int Hq,
-                                  int splits) {
+// out[r, h, :] = sum over ranges of 2^(lse - max) part / sum of 2^(lse - max); a row without keys: zeros.  A warp a head: a lane knows one
+// range's weight, and only the ranges that have keys are read.
+__global__ void __launch_bounds__(128)
+beams_join_kernel(const float* part_o, const float* part_lse, bf16* out, int out_stride, int Hq, int splits, int heads) {
     pdl_wait();
-    const int r = blockIdx.x, h = blockIdx.y;
-    const size_t p = ((size_t)r * Hq + h) * splits;
-    float M = -INFINITY;
-    for (int s = 0; s < splits; ++s) M = fmaxf(M, part_lse[p + s]);
-    for (int d = threadIdx.x; d < HD; d += blockDim.x) {
-        float W = 0.f, O = 0.f;
-        for (int s = 0; s < splits; ++s) {
-            const float lse = part_lse[p + s];
-            if (lse == -INFINITY) continue;                // a range without keys
-            const float w = exp2f(lse - M);
-            W += w;
-            O += w * part_o[(p + s) * HD + d];
+    const int id = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (id >= heads) return;
+    const size_t p = (size_t)id * splits;
+    const float lse = lane < splits ? part_lse[p + lane] : -INFINITY;
+    const float M = warp_max(lse);
+    float w = lse == -INFINITY ? 0.f : exp2f(lse - M);
+    w /= warp_sum(w);                                      // (nothing at all: no range is read)
+    constexpr int V = (HD + 127) / 128;                    // fours a lane
+    float4 v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (unsigned some = __ballot_sync(0xffffffffu, lse != -INFINITY); some;) {
+        // two ranges' loads in flight together
+        const int s0 = __ffs(some) - 1;
+        some &= some - 1;
+        const int s1 = some ? __ffs(some) - 1 : -1;
+        some &= some - 1;
+        const float w0 = __shfl_sync(0xffffffffu, w, s0), w1 = __shfl_sync(0xffffffffu, w, max(0, s1));
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int d = lane * 4 + i * 128;
+            if (d < HD) {
+                const float4 x = *reinterpret_cast<const float4*>(part_o + (p + s0) * HD + d);
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (s1 >= 0) y = *reinterpret_cast<const float4*>(part_o + (p + s1) * HD + d);
+                v[i].x += w0 * x.x; v[i].y += w0 * x.y; v[i].z += w0 * x.z; v[i].w += w0 * x.w;
+                if (s1 >= 0) { v[i].x += w1 * y.x; v[i].y += w1 * y.y; v[i].z += w1 * y.z; v[i].w += w1 * y.w; }
+            }
         }
-        out[(size_t)r * out_stride + (size_t)h * HD + d] = __float2bfloat16_rn(W == 0.f ? 0.f : O / W);
+    }
+    const int r = id / Hq, h = id - r * Hq;
+    bf16* to = out + (size_t)r * out_stride + (size_t)h * HD;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int d = lane * 4 + i * 128;
+        if (d < HD) {
+            to[d] = __float2bfloat16_rn(v[i].x);
+            to[d + 1] = __float2bfloat16_rn(v[i].y);
+            to[d + 2] = __float2bfloat16_rn(v[i].z);
+            to[d + 3] = __float2bfloat16_rn(v[i].w);
+        }
     }
 }
 
-constexpr size_t smem_bytes(int rtiles) {
-    const size_t kv = (size_t)STAGES * 2 * KT * ROW * sizeof(bf16), merge = (WARPS * 16 * (size_t)HD + 2 * WARPS * 16) * sizeof(float);
-    return (size_t)rtiles * 16 * ROW * sizeof(bf16) + (kv > merge ? kv : merge);
+template <int RTILES, bool TMA>
+constexpr size_t smem_bytes() {
+    const size_t kv = (size_t)STAGES * 2 * tile_keys<RTILES>() * (TMA ? HD : ROW) * sizeof(bf16) + (size_t)RTILES * 16 * ROW * sizeof(bf16) + 64;
+    const size_t merge = (WARPS * 16 * (size_t)OROW + 2 * WARPS * 16) * sizeof(float), own = (size_t)WARPS * 2 * OWN_KEYS * ROW * sizeof(bf16);
+    return 1024 /*alignment*/ + (kv > merge ? (kv > own ? kv : own) : (merge > own ? merge : own));
 }
-template <int RTILES>
-int run(const Args& a, int groups, cudaStream_t stream) {
-    static int configured = -1;
-    if (configured != 0) {
-        configured = (int)cudaFuncSetAttribute(beams_kernel<RTILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(RTILES));
-        if (configured != 0) return configured;
+
+// One layer of the cache, [page][K|V][kv head][slot][HD], seen as a matrix of HD-wide rows, in boxes of 64 columns x box_rows rows with the
+// 128-byte swizzle.
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+int cache_map(const void* ptr, long long rows, int box_rows, CUtensorMap* out) {
+    static std::mutex mu;
+    static EncodeTiledFn fn = nullptr;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        if (!fn) {
+            void* sym = nullptr;
+            cudaDriverEntryPointQueryResult q;
+            if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+                return (int)cudaErrorNotSupported;
+            fn = reinterpret_cast<EncodeTiledFn>(sym);
+        }
     }
-    const int G = a.Hq / a.Hkv, chunks = (a.beams * G + RTILES * 16 - 1) / (RTILES * 16), own_chunks = (G + 15) / 16;
-    const long long blocks = (long long)groups * a.Hkv * ((long long)chunks * a.shared_splits + (long long)a.beams * own_chunks * a.own_splits);
-    if (blocks > 0x7fffffffll) return (int)cudaErrorInvalidValue;
-    return ri_launch(beams_kernel<RTILES>, dim3((unsigned)blocks), dim3(THREADS), smem_bytes(RTILES), stream, a, groups, chunks, own_chunks);
+    cuuint64_t dims[2] = {(cuuint64_t)HD, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)HD * 2};
+    cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, elem[2] = {1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? 0
+               : (int)cudaErrorInvalidValue;
+}
+
+template <int RTILES, bool TMA>
+int run(Args a, long long pages, cudaStream_t stream) {
+    constexpr int bytes = (int)smem_bytes<RTILES, TMA>();
+    RI_CHECKED((int)cudaFuncSetAttribute(beams_kernel<RTILES, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    CUtensorMap map = {};
+    if constexpr (TMA) {
+        a.box_rows = a.page_size < tile_keys<RTILES>() ? a.page_size : tile_keys<RTILES>() == 128 && a.page_size % 128 ? 64 : tile_keys<RTILES>();
+        RI_CHECKED(cache_map(a.cache, pages * 2 * a.Hkv * a.page_size, a.box_rows, &map));
+    }
+    const int G = a.Hq / a.Hkv, chunks = (a.beams * G + RTILES * 16 - 1) / (RTILES * 16), own_chunks = (G + 7) / 8;
+    const long long units = (long long)a.groups * a.beams * a.Hkv * own_chunks * a.own_splits;
+    const long long blocks = (long long)a.groups * a.Hkv * chunks * a.shared_splits + (units + WARPS - 1) / WARPS;
+    if (blocks * WARPS > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+    return ri_launch(beams_kernel<RTILES, TMA>, dim3((unsigned)blocks), dim3(THREADS), (size_t)bytes, stream, map, a, chunks, own_chunks);
+}
+bool by_tma(const void* cache, int page_size, long long pages, int Hkv) {
+    return BY_TMA && (page_size == 8 || page_size == 16 || page_size == 32 || page_size % 64 == 0) && (reinterpret_cast<uintptr_t>(cache) & 15) == 0 &&
+           pages * 2 * Hkv * page_size < (1ll << 31);     // rows are 32-bit coordinates
+}
+template <bool TMA>
+int run_rows(const Args& a, long long pages, cudaStream_t s) {
+    const int rows = a.beams * (a.Hq / a.Hkv);
+    return rows <= 16 ? run<1, TMA>(a, pages, s) : rows <= 32 ? run<2, TMA>(a, pages, s) : run<4, TMA>(a, pages, s);
 }
 }  // namespace
 
 // Row tiles of 16 a CTA takes of a group's beams x heads
 RI_API int ri_attention_beams_row_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
-RI_API int ri_attention_beams_ctas_per_sm(int row_tiles) {
-    const int n = (int)(227 * 1024 / (smem_bytes(row_tiles) + 1024));
-    return n < 1 ? 1 : n < 2048 / THREADS ? n : 2048 / THREADS;
-}
+RI_API int ri_attention_beams_ctas_per_sm() { return CTAS; }
 
-// part_o: rows * Hq * (shared_splits + own_splits) * HD floats, part_lse the same without HD.
-RI_API int ri_attention_beams(const void* q, int q_stride, void* out, int out_stride, const void* cache, const int* table, int table_stride, int table_cols,
-                              const int* kv_len, const int* shared_len, int groups, int beams, int Hq, int Hkv, int page_size, float scale,
-                              int window, int shared_splits, int own_splits, float* part_o, float* part_lse, void* stream) {
+// part_o: rows * Hq * (shared_splits + own_splits) * HD floats, part_lse the same without HD.  `error` gets 22 where a wait for a copy ran out.
+RI_API int ri_attention_beams(const void* q, int q_stride, void* out, int out_stride, const void* cache, long long pages, const int* table,
+                              int table_stride, int table_cols, const int* kv_len, const int* shared_len, int groups, int beams, int Hq, int Hkv,
+                              int page_size, float scale, int window, int shared_splits, int own_splits, int target, float* part_o, float* part_lse,
+                              int* error, void* stream) {
     if (groups <= 0) return 0;
-    if (beams < 1 || beams > MAX_BEAMS || Hkv <= 0 || Hq % Hkv != 0 || Hq > 65535 || page_size < 1 || shared_splits < 1 || own_splits < 1 || !part_o ||
-        !part_lse)
+    if (beams < 1 || beams > MAX_BEAMS || Hkv <= 0 || Hq % Hkv != 0 || page_size < 1 || shared_splits < 1 || own_splits < 1 ||
+        shared_splits + own_splits > 32 || !part_o || !part_lse || !error || (long long)groups * beams * Hq > 0x7fffffffll)
         return (int)cudaErrorInvalidValue;
-    const Args a{(const bf16*)q, q_stride, (const bf16*)cache, table, table_stride,
-                 (int)min((long long)table_cols * page_size, 0x7fffffffll - KT), kv_len, shared_len, beams, Hq, Hkv, page_size,
-                 scale * 1.4426950408889634f, window, shared_splits, own_splits, part_o, part_lse};
+    const Args a{(const bf16*)q, q_stride, (const bf16*)cache, table, table_stride, (int)min((long long)table_cols * page_size, 0x7fffffffll - 256),
+                 kv_len, shared_len, beams, Hq, Hkv, page_size, scale * 1.4426950408889634f, window, groups, shared_splits, own_splits,
+                 target < 1 ? 1 : target, part_o, part_lse, error, 8};
     cudaStream_t s = (cudaStream_t)stream;
-    const int tiles = ri_attention_beams_row_tiles(beams * (Hq / Hkv));
-    RI_CHECKED(tiles == 1 ? run<1>(a, groups, s) : tiles == 2 ? run<2>(a, groups, s) : run<4>(a, groups, s));
-    RI_CHECKED(ri_launch(beams_join_kernel, dim3(groups * beams, Hq), dim3(HD < 128 ? 64 : 128), 0, s, part_o, part_lse, (bf16*)out, out_stride, Hq,
-                         shared_splits + own_splits));
+    bool tma = false;
+    if constexpr (BY_TMA) {
+        tma = by_tma(cache, page_size, pages, Hkv);
+        if (tma) RI_CHECKED(run_rows<true>(a, pages, s));
+    }
+    if (!tma) RI_CHECKED(run_rows<false>(a, pages, s));
+    const int heads = groups * beams * Hq;
+    RI_CHECKED(ri_launch(beams_join_kernel, dim3((heads + 3) / 4), dim3(128), 0, s, part_o, part_lse, (bf16*)out, out_stride, Hq,
+                         shared_splits + own_splits, heads));
     return ri_launch_status();
 }
 

@@ -2143,17 +2143,20 @@ def attention_beams_supports(num_heads: int, num_kv_heads: int, head_dim: int) -
 
 
 @functools.lru_cache(maxsize=4096)
+def _attention_beams_plan(rows: int, beams: int, num_heads: int, num_kv_heads: int, head_dim: int, most_shared: int, most_own: int,
+                          num_sms: int) -> Tuple[int, int, int]:
+    """`attention_beams_splits`, and how many CTAs the shared keys are cut for: what the SMs hold at once."""
+    lib = L.attention_beams(head_dim)
+    return (*attention_beams_splits(rows, beams, num_heads, num_kv_heads, head_dim, most_shared, most_own, num_sms),
+            int(lib.ri_attention_beams_ctas_per_sm()) * num_sms)
+
+
+@functools.lru_cache(maxsize=4096)
 def attention_beams_splits(rows: int, beams: int, num_heads: int, num_kv_heads: int, head_dim: int, most_shared: int, most_own: int,
                            num_sms: int) -> Tuple[int, int]:
-    """Ranges that the shared keys of a group, and the keys of a row's own, are cut into (16 at most in all, for scratch that is made for
-    `GQAAttention.MAX_SPLITS`): about a wave of CTAs for the former."""
-    lib = L.attention_beams(head_dim)
-    group = num_heads // num_kv_heads
-    row_tiles = int(lib.ri_attention_beams_row_tiles(beams * group))
-    slots = int(lib.ri_attention_beams_ctas_per_sm(row_tiles)) * num_sms
-    ctas = rows // beams * num_kv_heads * -(-beams * group // (16 * row_tiles))
-    shared = max(1, min(slots // max(1, ctas), -(-most_shared // 128), 12))
-    return shared, max(1, min(-(-most_own // 256), 4))
+    """Ranges there is room for of a group's shared keys, and ranges a row's own keys are cut into (16 at most in all, for scratch that
+    is made for `GQAAttention.MAX_SPLITS`)."""
+    return max(1, min(-(-most_shared // 64), 12)), max(1, min(-(-most_own // 32), 4))
 
 
 def attention_decode_beams(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,
@@ -2189,18 +2192,18 @@ def attention_decode_beams(q: torch.Tensor, out: torch.Tensor, cache: torch.Tens
     _contig(cache, "cache"); _contig(kv_len, "kv_len"); _contig(shared_len, "shared_len")
     if block_table.dim() != 2 or block_table.shape[0] < R or block_table.stride(1) != 1 or kv_len.numel() < R or shared_len.numel() < R // beams:
         raise KernelError(f"attention_decode_beams: a block table and a length for {R} rows, a shared length for {R // beams} groups")
-    if window is not None and window < 1:
-        raise KernelError(f"attention_decode_beams: a window of {window} keys")
+    if (window is not None and window < 1) or not scale > 0 or scale == math.inf:
+        raise KernelError(f"attention_decode_beams: a window of {window} keys, a scale of {scale}")
     if R == 0:
         return
-    splits = attention_beams_splits(R, beams, num_heads, num_kv_heads, head_dim, max(0, int(most_shared)), max(1, int(most_own)), L.num_sms(q.device))
-    need_o, need_l = decode_scratch_floats(R, num_heads, head_dim, sum(splits))
+    splits = _attention_beams_plan(R, beams, num_heads, num_kv_heads, head_dim, max(0, int(most_shared)), max(1, int(most_own)), L.num_sms(q.device))
+    need_o, need_l = decode_scratch_floats(R, num_heads, head_dim, splits[0] + splits[1])
     if part_o is None or part_lse is None:
         scratch = torch.empty(need_o + need_l, dtype=torch.float32, device=q.device)
         part_o, part_lse = scratch[:need_o], scratch[need_o:]
     if part_o.dtype != torch.float32 or part_lse.dtype != torch.float32 or part_o.numel() < need_o or part_lse.numel() < need_l:
         raise KernelError(f"attention_decode_beams: scratch must hold {need_o} and {need_l} fp32")
     check(L.attention_beams(head_dim).ri_attention_beams(
-        _p(q), q.stride(0), _p(out), out.stride(0), _p(cache), _p(block_table), block_table.stride(0), block_table.shape[1], _p(kv_len),
-        _p(shared_len), R // beams, beams, num_heads, num_kv_heads, cache.shape[3], float(scale), int(window or 0), splits[0], splits[1], _p(part_o),
-        _p(part_lse), stream_ptr()), "attention_decode_beams", 2)
+        _p(q), q.stride(0), _p(out), out.stride(0), _p(cache), cache.shape[0], _p(block_table), block_table.stride(0), block_table.shape[1], _p(kv_len),
+        _p(shared_len), R // beams, beams, num_heads, num_kv_heads, cache.shape[3], float(scale), int(window or 0), *splits, _p(part_o),
+        _p(part_lse), _p(gemm_tc_state(q.device)[2]), stream_ptr()), "attention_decode_beams", 2)

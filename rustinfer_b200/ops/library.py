@@ -102,9 +102,9 @@ _SIGNATURES = {
     "ri_beam_select": [_P, _L, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P],
     "ri_reorder_rows": [_P, _I, _L, _L, _L, _L, _P, _P, _I, _I, _P, _P],
     "ri_copy_pages": [_P, _I, _L, _L, _L, _L, _P, _P, _I, _P, _P],
-    "ri_attention_beams": [_P, _I, _P, _I, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _I, _P, _P, _P],
+    "ri_attention_beams": [_P, _I, _P, _I, _P, _L, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _I, _I, _P, _P, _P, _P],
     "ri_attention_beams_row_tiles": [_I],
-    "ri_attention_beams_ctas_per_sm": [_I],
+    "ri_attention_beams_ctas_per_sm": [],
     "ri_gated_decay": [_P, _P, _I, _F, _I, _I, _P],
     "ri_delta_prepare": [_P, _I, _P, _I, _P, _P, _P, _I, _I, _F, _F, _P, _P, _I, _I, _I, _P],
 }

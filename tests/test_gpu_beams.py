@@ -434,7 +434,7 @@ def test_attention_of_beams_refuses(K):
         a.update(kw)
         return lambda: K.attention_decode_beams(**a)
     call()()
-    for kw in (dict(q=q.float()), dict(beams=3), dict(beams=65), dict(beams=0), dict(num_heads=3), dict(head_dim=24), dict(head_dim=272), dict(window=0),
+    for kw in (dict(q=q.float()), dict(beams=3), dict(beams=65), dict(beams=0), dict(num_heads=3), dict(head_dim=24), dict(head_dim=272), dict(window=0), dict(scale=0.0), dict(scale=math.nan),
                dict(cache=cache.float()), dict(cache=cache[:, :, :1]), dict(kv_len=kv_len.long()), dict(kv_len=kv_len[:3]), dict(shared_len=sh[:1]),
                dict(block_table=table[:3]), dict(block_table=table.long()), dict(out=torch.empty((4, 255), dtype=torch.bfloat16, device="cuda")),
                dict(q=torch.zeros((4, 264), dtype=torch.bfloat16, device="cuda")[:, 1: 257]), dict(q=q.cpu()),
