@@ -189,16 +189,13 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
     const int boxes = KT / a.box_rows;                     // of keys, of 64 columns
     constexpr int MOST_BOXES = 2 * (KT / 8) * (BY_TMA ? TKB : 1);
     constexpr int TURNS = (MOST_BOXES + 31) / 32;          // (pages of 8 keys: more boxes than lanes)
-    int row_of[TURNS];
+    int page_of[TURNS];                                    // (as it was read: nothing waits for the load before the fetch does)
     auto look_up_boxes = [&](int t) {
 #pragma unroll
         for (int i = 0; i < TURNS; ++i) {
             const int box = lane + 32 * i, kv = box / (boxes * TKB), c = (box - kv * boxes * TKB) / TKB, key = (t0 + t) * KT + c * a.box_rows;
-            row_of[i] = -1;                                // boxes without a key in [lo, hi) are not fetched
-            if (box < 2 * boxes * TKB && key < hi && key + a.box_rows > lo) {
-                const int blk = key / a.page_size;
-                row_of[i] = ((bt[blk] * 2 + kv) * a.Hkv + kvh) * a.page_size + (key - blk * a.page_size);
-            }
+            page_of[i] = -1;                               // boxes without a key in [lo, hi) are not fetched
+            if (box < 2 * boxes * TKB && key < hi && key + a.box_rows > lo) page_of[i] = bt[key / a.page_size];
         }
     };
     auto fetch = [&](int t, int stage) {                   // tile t, which was looked up; looks up the next
@@ -206,16 +203,17 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
             if (warp == 0) {
                 int mine = 0;
 #pragma unroll
-                for (int i = 0; i < TURNS; ++i) mine += row_of[i] >= 0;
+                for (int i = 0; i < TURNS; ++i) mine += page_of[i] >= 0;
                 const int all = __reduce_add_sync(0xffffffffu, mine);
                 if (lane == 0) bar_expect(&full[stage], (unsigned)all * a.box_rows * 128);
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < TURNS; ++i) {
                     const int box = lane + 32 * i, kv = box / (boxes * TKB), rest = box - kv * boxes * TKB, c = rest / TKB, kb = rest - c * TKB;
-                    if (row_of[i] >= 0)
+                    const int key = (t0 + t) * KT + c * a.box_rows;
+                    if (page_of[i] >= 0)
                         tma_load_2d(reinterpret_cast<unsigned char*>(KVs + stage * STAGE) + ((kv * TKB + kb) * KT + c * a.box_rows) * 128, map,
-                                    &full[stage], kb * 64, row_of[i]);
+                                    &full[stage], kb * 64, ((page_of[i] * 2 + kv) * a.Hkv + kvh) * a.page_size + key % a.page_size);
                 }
                 if (t + 1 < tiles) look_up_boxes(t + 1);
             }
@@ -436,14 +434,15 @@ __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, i
     bf16* Vs = Ks + OWN_KEYS * ROW;
     const int* bt = a.table + (size_t)r * a.table_stride;
     const size_t head_step = (size_t)a.page_size * HD, value_step = (size_t)a.Hkv * head_step;
-    auto fetch = [&](bf16* to, int k0, size_t step) {      // a lane a row's half: 16 rows, two lanes each
-        const int kk = lane >> 1, key = k0 + kk;
-        const bool there = key < hi;
-        const bf16* src = a.cache;
-        if (there) {
-            const int blk = key / a.page_size;
-            src = a.cache + ((size_t)bt[blk] * 2 * a.Hkv + kvh) * head_step + (size_t)(key - blk * a.page_size) * HD + step;
-        }
+    // a lane's half of a row, 16 rows, two lanes each; its page's number is read a step ahead
+    auto look_up = [&](int k0) -> int {
+        const int key = k0 + (lane >> 1);
+        return key < hi ? bt[key / a.page_size] : -1;
+    };
+    auto fetch = [&](bf16* to, int k0, int page, size_t step) {
+        const int kk = lane >> 1;
+        const bool there = k0 + kk < hi;
+        const bf16* src = there ? a.cache + ((size_t)page * 2 * a.Hkv + kvh) * head_step + (size_t)((k0 + kk) % a.page_size) * HD + step : a.cache;
 #pragma unroll
         for (int ch = 0; ch < CH / 2; ++ch) {
             const int c = 2 * ch + (lane & 1);
@@ -456,8 +455,9 @@ __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, i
         if (lane < heads) a.part_lse[p0 + (size_t)lane * splits] = -INFINITY;
         return;
     }
-    fetch(Ks, lo, 0);
-    fetch(Vs, lo, value_step);
+    int page = look_up(lo), page_then = look_up(lo + OWN_KEYS);
+    fetch(Ks, lo, page, 0);
+    fetch(Vs, lo, page, value_step);
     unsigned qf[KS][2];                                    // rows 0 to 7 alone
     {
         const int h = lane >> 2;
@@ -484,7 +484,9 @@ __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, i
             mma_8rows(s[1], qf[ks][0], qf[ks][1], kf[2], kf[3]);
         }
         __syncwarp();
-        if (k0 + OWN_KEYS < hi) fetch(Ks, k0 + OWN_KEYS, 0);
+        page = page_then;
+        page_then = look_up(k0 + 2 * OWN_KEYS);
+        if (k0 + OWN_KEYS < hi) fetch(Ks, k0 + OWN_KEYS, page, 0);
         else cp_async_commit();
         float mx = -INFINITY;
 #pragma unroll
@@ -523,7 +525,7 @@ __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, i
             mma_8rows(o[2 * np + 1], pl[0], pl[1], vf[2], vf[3]);
         }
         __syncwarp();
-        if (k0 + OWN_KEYS < hi) fetch(Vs, k0 + OWN_KEYS, value_step);
+        if (k0 + OWN_KEYS < hi) fetch(Vs, k0 + OWN_KEYS, page, value_step);
         else cp_async_commit();
     }
     cp_async_wait<0>();
@@ -540,20 +542,32 @@ __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, i
     }
 }
 
-// Tiles of shared keys a CTA takes: as many as make about `target` CTAs of all groups' tiles together, and no more ranges of the longest
-// than there is room for
+// Tiles of shared keys a CTA takes: the fewest that leave all groups' ranges together no more CTAs than the `target` that run at once, and the
+// longest group no more ranges than there is room for
 __device__ __forceinline__ int tiles_a_range(const Args& a, int ctas_a_range, int KT) {
     const int lane = threadIdx.x & 31;
-    int total = 0, most = 0;
-    for (int g = lane; g < a.groups; g += 32) {
+    auto tiles_of = [&](int g) {
         const int n = keys_of(a, g * a.beams), lo = a.window > 0 ? max(0, n - a.window) : 0, hi = max(lo, min(a.shared_len[g], n));
-        const int tiles = (hi + KT - 1) / KT - lo / KT;
-        total += tiles;
-        most = max(most, tiles);
+        return hi > lo ? (hi + KT - 1) / KT - lo / KT : 0;
+    };
+    const int first = lane < a.groups ? tiles_of(lane) : 0;        // (a group a lane is read once)
+    int total = first, most = first;
+    for (int g = lane + 32; g < a.groups; g += 32) {
+        const int n = tiles_of(g);
+        total += n;
+        most = max(most, n);
     }
     total = __reduce_add_sync(0xffffffffu, total);
     most = __reduce_max_sync(0xffffffffu, most);
-    return max(1, max((int)(((long long)total * ctas_a_range + a.target - 1) / a.target), (most + a.shared_splits - 1) / a.shared_splits));
+    const int ranges = max(1, a.target / ctas_a_range);
+    int per = max(1, max((total + ranges - 1) / ranges, (most + a.shared_splits - 1) / a.shared_splits));
+    while (per < most) {
+        int n = (first + per - 1) / per;
+        for (int g = lane + 32; g < a.groups; g += 32) n += (tiles_of(g) + per - 1) / per;
+        if (__reduce_add_sync(0xffffffffu, n) <= ranges) break;
+        per += (per >> 3) + 1;
+    }
+    return per;
 }
 
 // Blocks: first (range of shared keys, group, key head, row chunk), then a warp for (range of the row's own keys, row, key head, eight heads).
@@ -685,7 +699,13 @@ int cache_map(const void* ptr, long long rows, int box_rows, CUtensorMap* out) {
 template <int RTILES, bool TMA>
 int run(Args a, long long pages, cudaStream_t stream) {
     constexpr int bytes = (int)smem_bytes<RTILES, TMA>();
-    RI_CHECKED((int)cudaFuncSetAttribute(beams_kernel<RTILES, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    static unsigned long long configured = 0;              // devices, a bit each (one that is set twice is set to the same)
+    int device = 0;
+    RI_CHECKED((int)cudaGetDevice(&device));
+    if (device > 63 || !(configured >> device & 1)) {
+        RI_CHECKED((int)cudaFuncSetAttribute(beams_kernel<RTILES, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        if (device <= 63) configured |= 1ull << device;
+    }
     CUtensorMap map = {};
     if constexpr (TMA) {
         a.box_rows = a.page_size < tile_keys<RTILES>() ? a.page_size : tile_keys<RTILES>() == 128 && a.page_size % 128 ? 64 : tile_keys<RTILES>();

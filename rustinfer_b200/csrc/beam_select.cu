@@ -566,7 +566,13 @@ RI_API int ri_beam_select(const float* logits, long long ld, int vocab, const fl
     unsigned long long* best = (unsigned long long*)(stat + (size_t)rows * slices);
     cudaStream_t s = (cudaStream_t)stream;
     constexpr int ring = STAGES * NV * (ST / 32) * 33 * 16;
-    RI_CHECKED((int)cudaFuncSetAttribute(beam_slices_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring));
+    static unsigned long long configured = 0;              // devices, a bit each (one that is set twice is set to the same)
+    int device = 0;
+    RI_CHECKED((int)cudaGetDevice(&device));
+    if (device > 63 || !(configured >> device & 1)) {
+        RI_CHECKED((int)cudaFuncSetAttribute(beam_slices_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring));
+        if (device <= 63) configured |= 1ull << device;
+    }
     RI_CHECKED(ri_launch(beam_slices_kernel, dim3(min(rows * slices, CTAS * sms)), dim3(ST), ring, s, logits, ld, vocab, scores, picks, rows * slices,
                          slices, a_slice, best, stat));
     RI_CHECKED(ri_launch(beam_merge_kernel, dim3(groups), dim3(MT), 0, s, best, stat, scores, vocab, beams, slices, picks, out_scores, out_rows,

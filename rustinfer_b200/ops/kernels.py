@@ -2031,12 +2031,23 @@ def sample_scratch_elems(rows: int, vocab: int) -> int:
 BEAMS_MAX, BEAM_PICKS_MAX = 64, 128
 
 
-def _on_current_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    """Kernels are launched on the current device's stream: tensors of another one are refused, not reached over its back."""
-    current = L._current_device()
+def _here(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """CUDA tensors of the current device: a kernel is launched on its stream, and a tensor of another one is refused, not reached over
+    its back."""
+    current = L._current_device() if torch.cuda.is_initialized() else -2
     for t in tensors:
         if t is not None and t.get_device() != current:
-            raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{current}")
+            raise KernelError(f"{what}: a tensor on {t.device}; the sm_100a kernels take tensors of the current CUDA device only, there is no CPU path")
+
+
+def _vec(t: torch.Tensor, n: int, dtype: torch.dtype, what: str) -> None:
+    if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        raise KernelError(f"{what} is contiguous {dtype} with {n} elements, got {t.dtype} {tuple(t.shape)}")
+
+
+@functools.lru_cache(maxsize=4096)
+def _beam_slices(rows: int, vocab: int, num_sms: int) -> int:
+    return int(L.beams().ri_beam_select_slices(rows, vocab, num_sms))
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, out_scores: torch.Tensor, out_rows: torch.Tensor,
@@ -2048,50 +2059,45 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, out_scor
     tokens (int32).  Equal scores go by ascending (row, token); scores are compared in 64 bits.  A row whose score is -inf
     has no continuation but of score -inf, and neither has a token whose logit is -inf or not a number.  In a row that
     holds +inf, those tokens share the weight.  Up to 64 beams and 128 picks."""
-    require_cuda(logits, scores, out_scores, out_rows, out_tokens)
-    _on_current_device("beam_select", logits, scores, out_scores, out_rows, out_tokens)
+    _here("beam_select", logits, scores, out_scores, out_rows, out_tokens)
     if logits.dtype != torch.float32 or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise KernelError("beam_select: logits are fp32 [rows, vocab] with unit column stride")
     R, V = logits.shape
     if not 1 <= beams <= BEAMS_MAX or R % beams:
         raise KernelError(f"beam_select: {R} rows are no groups of {beams} (1 to {BEAMS_MAX})")
-    if scores.dtype != torch.float32 or scores.numel() != R:
-        raise KernelError(f"beam_select: scores are fp32 [{R}]")
-    groups = R // beams
-    picks = out_scores.shape[-1]
-    for t, n, dt in ((out_scores, "out_scores", torch.float32), (out_rows, "out_rows", torch.int32), (out_tokens, "out_tokens", torch.int32)):
-        if t.dtype != dt or t.shape != (groups, picks):
-            raise KernelError(f"beam_select: {n} is {dt} [{groups}, {picks}], got {t.dtype} {tuple(t.shape)}")
-        _contig(t, n)
-    _contig(scores, "scores")
+    groups, picks = R // beams, out_scores.shape[-1] if out_scores.dim() else 0
     if not 1 <= picks <= min(BEAM_PICKS_MAX, beams * V):
         raise KernelError(f"beam_select: {picks} picks of {beams} x {V} continuations (1 to {BEAM_PICKS_MAX})")
+    _vec(scores, R, torch.float32, "beam_select: scores")
+    _vec(out_scores, groups * picks, torch.float32, "beam_select: out_scores")
+    _vec(out_rows, groups * picks, torch.int32, "beam_select: out_rows")
+    _vec(out_tokens, groups * picks, torch.int32, "beam_select: out_tokens")
     if R == 0:
         return
     if R > 65535 or V > 1 << 30:
         raise KernelError(f"beam_select: {R} rows of {V} tokens (up to 65,535 rows and 2^30 tokens)")
-    lib, sms = L.beams(), L.num_sms(logits.device)
+    sms = L.num_sms(logits.device)
     # a sum (16 bytes) and the best (8 each, twice `picks` at most) of every slice of every row
-    scratch = torch.empty(R * lib.ri_beam_select_slices(R, V, sms) * (2 + 2 * picks), dtype=torch.int64, device=logits.device)
-    check(lib.ri_beam_select(_p(logits), logits.stride(0), V, _p(scores), groups, beams, picks, sms, _p(scratch), _p(out_scores), _p(out_rows),
-                             _p(out_tokens), stream_ptr()), "beam_select", 2)
+    scratch = torch.empty(R * _beam_slices(R, V, sms) * (2 + 2 * picks), dtype=torch.int64, device=logits.device)
+    check(L.beams().ri_beam_select(logits.data_ptr(), logits.stride(0), V, scores.data_ptr(), groups, beams, picks, sms, scratch.data_ptr(),
+                                   out_scores.data_ptr(), out_rows.data_ptr(), out_tokens.data_ptr(), stream_ptr()), "beam_select", 2)
 
 
 def _row_sizes(what: str, store: torch.Tensor, tokens: Optional[torch.Tensor], n: int) -> Tuple[int, int, int, int, int]:
     """(layers, rows, bytes a row, bytes a segment, bytes a token) of a cache's storage."""
-    if store.dim() < 2:
-        raise KernelError(f"{what}: the storage is [layers, rows, ...], got {tuple(store.shape)}")
-    _contig(store, "store")
-    layers, total = store.shape[:2]
-    row = store[0, 0].numel() * store.element_size() if store.numel() else 0
+    shape = store.shape
+    if len(shape) < 2 or not store.is_contiguous():
+        raise KernelError(f"{what}: the storage is contiguous [layers, rows, ...], got {tuple(shape)}")
+    row = math.prod(shape[2:]) * store.element_size()
+    if row >= 1 << 31 or shape[0] > 65535:
+        raise KernelError(f"{what}: {shape[0]} layers, rows of {row} bytes (below 65,536 and 2^31)")
     if tokens is None:
-        return layers, total, row, row, row
-    _i32(tokens, "tokens")
-    if store.dim() != 6 or store.shape[2] != 2 or tokens.numel() != n:
-        raise KernelError(f"{what}: tokens are int32 [{n}], for pages [layers, pages, 2, kv heads, page, head_dim]")
-    _contig(tokens, "tokens")
-    token = store.shape[5] * store.element_size()
-    return layers, total, row, store.shape[4] * token, token
+        return shape[0], shape[1], row, row, row
+    if len(shape) != 6 or shape[2] != 2:
+        raise KernelError(f"{what}: tokens are for pages [layers, pages, 2, kv heads, page, head_dim], got {tuple(shape)}")
+    _vec(tokens, n, torch.int32, f"{what}: tokens")
+    token = shape[5] * store.element_size()
+    return shape[0], shape[1], row, shape[4] * token, token
 
 
 def reorder_rows(store: torch.Tensor, rows: torch.Tensor, parents: torch.Tensor, beams: int, tokens: Optional[torch.Tensor] = None) -> None:
@@ -2102,19 +2108,19 @@ def reorder_rows(store: torch.Tensor, rows: torch.Tensor, parents: torch.Tensor,
     With `tokens` (int32 [groups * beams]) the storage is pages [layers, pages, 2, kv heads, page, head_dim], and only the
     first tokens[r] tokens of a page are taken over.  A parent outside the group and a row outside the storage leave the row
     as it is.  No row may be listed twice."""
-    require_cuda(store, rows, parents, tokens)
-    _on_current_device("reorder_rows", store, rows, parents, tokens)
-    _i32(rows, "rows"); _i32(parents, "parents"); _contig(rows, "rows"); _contig(parents, "parents")
+    _here("reorder_rows", store, rows, parents, tokens)
     n = rows.numel()
-    if not 1 <= beams <= BEAMS_MAX or n % beams or parents.numel() != n:
-        raise KernelError(f"reorder_rows: {n} rows and {parents.numel()} parents are no groups of {beams} (1 to {BEAMS_MAX})")
+    if not 1 <= beams <= BEAMS_MAX or n % beams:
+        raise KernelError(f"reorder_rows: {n} rows are no groups of {beams} (1 to {BEAMS_MAX})")
+    _vec(rows, n, torch.int32, "reorder_rows: rows")
+    _vec(parents, n, torch.int32, "reorder_rows: parents")
     layers, total, row, seg, token = _row_sizes("reorder_rows", store, tokens, n)
     if n == 0 or layers == 0 or row == 0 or total == 0:
         return
-    if layers > 65535 or n // beams > 65535 or row >= 1 << 31:
-        raise KernelError(f"reorder_rows: {layers} layers, {n // beams} groups, rows of {row} bytes (below 65,536, 65,536 and 2^31)")
-    check(L.beams().ri_reorder_rows(_p(store), layers, total, row, seg, token, _p(rows), _p(parents), n // beams, beams, _p(tokens), stream_ptr()),
-          "reorder_rows")
+    if n // beams > 65535:
+        raise KernelError(f"reorder_rows: {n // beams} groups (below 65,536)")
+    check(L.beams().ri_reorder_rows(store.data_ptr(), layers, total, row, seg, token, rows.data_ptr(), parents.data_ptr(), n // beams, beams,
+                                    _p(tokens), stream_ptr()), "reorder_rows")
 
 
 def copy_pages(store: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, tokens: Optional[torch.Tensor] = None) -> None:
@@ -2124,39 +2130,43 @@ def copy_pages(store: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, tokens
     [layers, pages, 2, kv heads, page, head_dim] and only the first tokens[i] tokens are copied.  A page outside the storage
     and a page copied to itself are left out.  A page may be the source of many copies; no page may be the destination of
     two, and no destination may be a source (the copies run side by side)."""
-    require_cuda(store, src, dst, tokens)
-    _on_current_device("copy_pages", store, src, dst, tokens)
-    _i32(src, "src"); _i32(dst, "dst"); _contig(src, "src"); _contig(dst, "dst")
+    _here("copy_pages", store, src, dst, tokens)
     n = src.numel()
-    if dst.numel() != n:
-        raise KernelError(f"copy_pages: {n} sources, {dst.numel()} destinations")
+    _vec(src, n, torch.int32, "copy_pages: src")
+    _vec(dst, n, torch.int32, "copy_pages: dst")
     layers, total, row, seg, token = _row_sizes("copy_pages", store, tokens, n)
     if n == 0 or layers == 0 or row == 0 or total == 0:
         return
-    if layers > 65535 or row >= 1 << 31:
-        raise KernelError(f"copy_pages: {layers} layers, pages of {row} bytes (below 65,536 and 2^31)")
-    check(L.beams().ri_copy_pages(_p(store), layers, total, row, seg, token, _p(src), _p(dst), n, _p(tokens), stream_ptr()), "copy_pages")
+    check(L.beams().ri_copy_pages(store.data_ptr(), layers, total, row, seg, token, src.data_ptr(), dst.data_ptr(), n, _p(tokens), stream_ptr()),
+          "copy_pages")
 
 
 def attention_beams_supports(num_heads: int, num_kv_heads: int, head_dim: int) -> bool:
     return num_kv_heads > 0 and num_heads % num_kv_heads == 0 and head_dim % 16 == 0 and 16 <= head_dim <= L.MMA_MAX_HEAD_DIM
 
 
+BEAM_SPLITS_MAX = 20          # ranges of a row's keys at most: 16 of shared ones, 4 of its own
+
+
+def attention_beams_splits(most_shared: int, most_own: int) -> Tuple[int, int]:
+    """Ranges there is room for of a group's shared keys, and ranges a row's own keys are cut into, for about so many keys."""
+    return max(1, min(-(-most_shared // 64), 16)), max(1, min(-(-most_own // 32), 4))
+
+
 @functools.lru_cache(maxsize=4096)
-def _attention_beams_plan(rows: int, beams: int, num_heads: int, num_kv_heads: int, head_dim: int, most_shared: int, most_own: int,
-                          num_sms: int) -> Tuple[int, int, int]:
-    """`attention_beams_splits`, and how many CTAs the shared keys are cut for: what the SMs hold at once."""
+def _attention_beams_plan(rows: int, beams: int, num_heads: int, num_kv_heads: int, head_dim: int, most_shared: int, most_own: int, num_sms: int):
+    """(entry point, ranges of shared keys, of own ones, CTAs for the former, floats of partial results and of their log-sum-exps).  The CTAs
+    that read shared keys are those that run at once, less a quarter of the ones that read the rows' own (4 x 16 beams of 9,001 and 300
+    keys: without the latter 71 us, less them all 84; 8 x 8 of 4,096 and 60: 35 and 42)."""
+    if not attention_beams_supports(num_heads, num_kv_heads, head_dim):
+        raise KernelError(f"attention_decode_beams: {num_heads} heads over {num_kv_heads} of {head_dim} (a multiple of 16 up to {L.MMA_MAX_HEAD_DIM})")
+    if not 1 <= beams <= BEAMS_MAX or rows % beams:
+        raise KernelError(f"attention_decode_beams: {rows} rows are no groups of {beams} (1 to {BEAMS_MAX})")
     lib = L.attention_beams(head_dim)
-    return (*attention_beams_splits(rows, beams, num_heads, num_kv_heads, head_dim, most_shared, most_own, num_sms),
-            int(lib.ri_attention_beams_ctas_per_sm()) * num_sms)
-
-
-@functools.lru_cache(maxsize=4096)
-def attention_beams_splits(rows: int, beams: int, num_heads: int, num_kv_heads: int, head_dim: int, most_shared: int, most_own: int,
-                           num_sms: int) -> Tuple[int, int]:
-    """Ranges there is room for of a group's shared keys, and ranges a row's own keys are cut into (16 at most in all, for scratch that
-    is made for `GQAAttention.MAX_SPLITS`)."""
-    return max(1, min(-(-most_shared // 64), 12)), max(1, min(-(-most_own // 32), 4))
+    shared, own = attention_beams_splits(most_shared, most_own)
+    at_once = int(lib.ri_attention_beams_ctas_per_sm()) * num_sms
+    own_ctas = -(-rows * num_kv_heads * -(-(num_heads // num_kv_heads) // 8) * own // 8)
+    return (lib.ri_attention_beams, shared, own, at_once - min(at_once // 4, own_ctas // 4), *decode_scratch_floats(rows, num_heads, head_dim, shared + own))
 
 
 def attention_decode_beams(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,
@@ -2168,42 +2178,43 @@ def attention_decode_beams(q: torch.Tensor, out: torch.Tensor, cache: torch.Tens
     pages they lie in.  These are read once for the group, by its first row's table.
 
     q, out bf16 [rows, heads * head_dim] (unit column stride), cache bf16 [pages, 2, kv heads, page, head_dim], block_table int32
-    [rows, pages a row], kv_len int32 [rows], shared_len int32 [rows / beams].  A row without keys gets zeros.  A group one of
-    whose rows has fewer keys than shared_len, or whose rows' windows start at different keys, is read row by row.
-    most_shared and most_own: about how many keys the longest shared part and the longest rest have (they choose how the work is
-    cut, not what is computed).  part_o, part_lse: fp32 scratch (`decode_scratch_floats` with the sum of
-    `attention_beams_splits`); without them it is allocated."""
-    require_cuda(q, out, cache, block_table, kv_len, shared_len, part_o, part_lse)
-    _on_current_device("attention_decode_beams", q, out, cache, block_table, kv_len, shared_len, part_o, part_lse)
-    for t, n in ((block_table, "block_table"), (kv_len, "kv_len"), (shared_len, "shared_len")):
-        _i32(t, n)
-    if not attention_beams_supports(num_heads, num_kv_heads, head_dim):
-        raise KernelError(f"attention_decode_beams: {num_heads} heads over {num_kv_heads} of {head_dim} (a multiple of 16 up to {L.MMA_MAX_HEAD_DIM})")
-    R = q.shape[0]
-    if not 1 <= beams <= BEAMS_MAX or R % beams:
-        raise KernelError(f"attention_decode_beams: {R} rows are no groups of {beams} (1 to {BEAMS_MAX})")
-    for t, n in ((q, "q"), (out, "out")):
-        if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape != (R, num_heads * head_dim) or t.stride(1) != 1 or t.stride(0) < t.shape[1]:
-            raise KernelError(f"attention_decode_beams: {n} is bf16 [{R}, {num_heads * head_dim}] with unit column stride")
-    if q.stride(0) % 8 or q.data_ptr() % 16 or cache.data_ptr() % 16:
+    [rows, pages a row] (a row has no more keys than its pages hold), kv_len int32 [rows], shared_len int32 [rows / beams].  A row
+    without keys gets zeros.  A group one of whose rows has fewer keys than shared_len, or whose rows' windows start at different
+    keys, is read row by row.  most_shared and most_own: about how many keys the longest shared part and the longest rest have
+    (they choose how the work is cut, not what is computed).  part_o, part_lse: fp32 scratch (`decode_scratch_floats` with the
+    sum of `attention_beams_splits`, at most BEAM_SPLITS_MAX); without them it is allocated."""
+    _here("attention_decode_beams", q, out, cache, block_table, kv_len, shared_len, part_o, part_lse)
+    R, width = q.shape[0], num_heads * head_dim
+    entry, shared, own, ctas, need_o, need_l = _attention_beams_plan(R, beams, num_heads, num_kv_heads, head_dim, max(0, int(most_shared)),
+                                                                     max(1, int(most_own)), L.num_sms(q.device))
+    bf16, i32 = torch.bfloat16, torch.int32
+    q_step, out_step = q.stride(0), out.stride(0)
+    if (q.dtype != bf16 or out.dtype != bf16 or q.shape != (R, width) or out.shape != (R, width) or q.stride(1) != 1 or out.stride(1) != 1
+            or (R > 1 and (q_step < width or out_step < width))):
+        raise KernelError(f"attention_decode_beams: q and out are bf16 [{R}, {width}] with unit column stride")
+    shape = cache.shape
+    if cache.dtype != bf16 or len(shape) != 5 or shape[1] != 2 or shape[2] != num_kv_heads or shape[4] != head_dim or not cache.is_contiguous():
+        raise KernelError("attention_decode_beams: cache is contiguous bf16 [pages, 2, kv heads, page, head_dim]")
+    q_ptr, cache_ptr = q.data_ptr(), cache.data_ptr()
+    if q_step % 8 or q_ptr % 16 or cache_ptr % 16:
         raise KernelError("attention_decode_beams: rows of q and the cache start on 16-byte boundaries")
-    if cache.dtype != torch.bfloat16 or cache.dim() != 5 or cache.shape[1] != 2 or cache.shape[2] != num_kv_heads or cache.shape[4] != head_dim:
-        raise KernelError("attention_decode_beams: cache is bf16 [pages, 2, kv heads, page, head_dim]")
-    _contig(cache, "cache"); _contig(kv_len, "kv_len"); _contig(shared_len, "shared_len")
-    if block_table.dim() != 2 or block_table.shape[0] < R or block_table.stride(1) != 1 or kv_len.numel() < R or shared_len.numel() < R // beams:
-        raise KernelError(f"attention_decode_beams: a block table and a length for {R} rows, a shared length for {R // beams} groups")
+    if (block_table.dtype != i32 or block_table.dim() != 2 or block_table.shape[0] < R or (block_table.shape[1] > 1 and block_table.stride(1) != 1)
+            or kv_len.dtype != i32 or shared_len.dtype != i32 or kv_len.numel() < R or shared_len.numel() < R // beams
+            or not kv_len.is_contiguous() or not shared_len.is_contiguous()):
+        raise KernelError(f"attention_decode_beams: an int32 block table and length for {R} rows, an int32 shared length for {R // beams} groups")
     if (window is not None and window < 1) or not scale > 0 or scale == math.inf:
         raise KernelError(f"attention_decode_beams: a window of {window} keys, a scale of {scale}")
     if R == 0:
         return
-    splits = _attention_beams_plan(R, beams, num_heads, num_kv_heads, head_dim, max(0, int(most_shared)), max(1, int(most_own)), L.num_sms(q.device))
-    need_o, need_l = decode_scratch_floats(R, num_heads, head_dim, splits[0] + splits[1])
     if part_o is None or part_lse is None:
         scratch = torch.empty(need_o + need_l, dtype=torch.float32, device=q.device)
-        part_o, part_lse = scratch[:need_o], scratch[need_o:]
-    if part_o.dtype != torch.float32 or part_lse.dtype != torch.float32 or part_o.numel() < need_o or part_lse.numel() < need_l:
-        raise KernelError(f"attention_decode_beams: scratch must hold {need_o} and {need_l} fp32")
-    check(L.attention_beams(head_dim).ri_attention_beams(
-        _p(q), q.stride(0), _p(out), out.stride(0), _p(cache), cache.shape[0], _p(block_table), block_table.stride(0), block_table.shape[1], _p(kv_len),
-        _p(shared_len), R // beams, beams, num_heads, num_kv_heads, cache.shape[3], float(scale), int(window or 0), *splits, _p(part_o),
-        _p(part_lse), _p(gemm_tc_state(q.device)[2]), stream_ptr()), "attention_decode_beams", 2)
+        o_ptr = scratch.data_ptr()
+        l_ptr = o_ptr + 4 * need_o
+    else:
+        if part_o.dtype != torch.float32 or part_lse.dtype != torch.float32 or part_o.numel() < need_o or part_lse.numel() < need_l \
+                or not part_o.is_contiguous() or not part_lse.is_contiguous() or part_o.data_ptr() % 16:
+            raise KernelError(f"attention_decode_beams: scratch is contiguous fp32, {need_o} and {need_l} elements, the former 16-byte aligned")
+        o_ptr, l_ptr = part_o.data_ptr(), part_lse.data_ptr()
+    check(entry(q_ptr, q_step, out.data_ptr(), out_step, cache_ptr, shape[0], block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+                kv_len.data_ptr(), shared_len.data_ptr(), R // beams, beams, num_heads, num_kv_heads, shape[3], scale, window or 0, shared, own, ctas,
+                o_ptr, l_ptr, gemm_tc_state(q.device)[2].data_ptr(), stream_ptr()), "attention_decode_beams", 2)

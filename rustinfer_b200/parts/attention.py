@@ -138,7 +138,7 @@ class GQAAttention(Mixer):
             self._tiles = token_tiles(self.tokens_per_tile, skip_single_token=True)
             key = ("decode_scratch", self.Hq, self.hd)
             if key not in ctx.shared:
-                no, nl = K.decode_scratch_floats(ctx.max_batch_seqs, self.Hq, self.hd, self.MAX_SPLITS)
+                no, nl = K.decode_scratch_floats(ctx.max_batch_seqs, self.Hq, self.hd, max(self.MAX_SPLITS, K.BEAM_SPLITS_MAX))
                 ctx.shared[key] = (torch.empty(no, dtype=torch.float32, device=ctx.device),
                                    torch.empty(nl, dtype=torch.float32, device=ctx.device))
             self.part_o, self.part_lse = ctx.shared[key]

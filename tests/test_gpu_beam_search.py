@@ -196,11 +196,12 @@ def test_forks_and_reorders_of_requests(folder, family, name, sizes):
 
 
 def test_requests_that_follow_a_search(folder):
-    """The scheduler's requests get what they get on an engine that never searched."""
+    """The scheduler's requests get what they get on an engine that never searched.  (In 32 bits: the bfloat16 engine's own tokens differ
+    now and then from run to run, without any search too, since its chained products add their slices in no fixed order.)"""
     from rustinfer_b200.engine.beam import BeamParams
     from rustinfer_b200.sampling.params import SamplingParams
     path = folder("llama", "D")
-    a, b = (_engine(path, "bfloat16", capture_sizes=[1, 2, 4]) for _ in range(2))
+    a, b = (_engine(path, "float32", capture_sizes=[1, 2, 4]) for _ in range(2))
     prompts = [random_ids(n, a.runner.spec.vocab_size, n) for n in (9, 40, 17)]
     a.beam_search(prompts, BeamParams(beams=4, max_tokens=8, ignore_eos=True))
     a.beam_search(prompts[:1], BeamParams(beams=6, max_tokens=8, ignore_eos=True))

@@ -416,7 +416,7 @@ def test_attention_of_beams_strides_scratch_and_hints(K):
     table = torch.nn.functional.pad(table.clamp(min=0), (0, 5, 0, 2))
     want = _attention(q, cache, table, kv_len, heads, kv_heads, dim, 0.125, None)
     for hints in ((700, 30), (0, 1), (100000, 100000)):
-        splits = K.attention_beams_splits(6, beams, heads, kv_heads, dim, hints[0], hints[1], 148)
+        splits = K.attention_beams_splits(*hints)
         a, b = K.decode_scratch_floats(6, heads, dim, sum(splits) + 1)
         K.attention_decode_beams(wide[:, 8: 8 + heads * dim], out[:, 1: 1 + heads * dim], cache, table, kv_len, sh, beams, heads, kv_heads, dim, 0.125,
                                  None, *hints, torch.empty(a, device="cuda"), torch.empty(b, device="cuda"))
