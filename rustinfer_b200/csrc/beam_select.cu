@@ -30,6 +30,7 @@ constexpr int CTAS = 3;                                    // CTAs an SM, which 
 constexpr int STAGES = 3;                                  // chunks of a slice in flight
 constexpr int MAX_CHUNKS = 8;                              // chunks of a slice
 constexpr int LISTS = 1024;                                // slices of a group whose sums are kept in shared memory
+constexpr int KEPT = 16384;                                // ... and elements of the pool whose rounded scores are
 constexpr int MT = 512;                                   // threads of a group
 constexpr int CAP = 1024;                                  // room of the gathering
 constexpr int MAX_PICKS = 128, MAX_BEAMS = 64;
@@ -368,6 +369,7 @@ __global__ void __launch_bounds__(MT)
 beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const float* scores,
                   int vocab, int beams, int slices, int picks, float* out_scores, int* out_rows,
                   int* out_tokens) {
+    extern __shared__ unsigned rounded[];                  // [lists][room], where they fit
     __shared__ double base[MAX_BEAMS], so_far[MAX_BEAMS];  // log of the row's sum; its score
     __shared__ float row_top[MAX_BEAMS];
     __shared__ double l_score[CAP];
@@ -434,7 +436,7 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
                 for (int q = 0; q < AT_ONCE; ++q) key[q] = k < n[q] ? keys[(size_t)(l0 + q * (MT / 32)) * room + k] : 0ull;
 #pragma unroll
                 for (int q = 0; q < AT_ONCE; ++q)
-                    if (key[q]) use((l0 + q * (MT / 32)) / slices, key[q]);
+                    if (key[q]) use((l0 + q * (MT / 32)) / slices, key[q], (l0 + q * (MT / 32)) * room + k);
             }
         }
     };
@@ -450,7 +452,12 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
     };
     // 32-bit keys for the search: rounding keeps the order, and equals after rounding are all gathered
     unsigned mine = 0;
-    each([&](int b, unsigned long long key) { mine = max(mine, ordered((float)score_of(b, key))); });
+    const bool kept = lists * room <= KEPT;
+    each([&](int b, unsigned long long key, int at) {
+        const unsigned o = ordered((float)score_of(b, key));
+        if (kept) rounded[at] = o;
+        mine = max(mine, o);
+    });
     unsigned top = __reduce_max_sync(0xffffffffu, mine);
     const unsigned low = __reduce_min_sync(0xffffffffu, mine ? mine : 0xffffffffu);
     if (lane == 0) { wmax[warp] = top; wmin[warp] = low; }
@@ -458,13 +465,21 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
     top = __reduce_max_sync(0xffffffffu, wmax[lane & (MT / 32 - 1)]);
     unsigned t = holders >= picks ? __reduce_min_sync(0xffffffffu, wmin[lane & (MT / 32 - 1)]) : 1;
     if (lists > 1) t = reach(mine, t, top, picks);
-    each([&](int b, unsigned long long key) {
-        const double s = score_of(b, key);
-        if (ordered((float)s) >= t) {
-            const int at = atomicAdd(&listed, 1);
-            if (at < CAP) { l_score[at] = s; l_flat[at] = flat_of(b, key); }
+    auto take = [&](int b, unsigned long long key) {
+        const int at = atomicAdd(&listed, 1);
+        if (at < CAP) { l_score[at] = score_of(b, key); l_flat[at] = flat_of(b, key); }
+    };
+    if (kept) {                                            // what reaches t is read again, the rest is not
+        for (int l = warp; l < lists; l += MT / 32) {
+            const int n = stat_of(l).n;
+            for (int k = lane; k < n; k += 32)
+                if (rounded[l * room + k] >= t) take(l / slices, keys[(size_t)l * room + k]);
         }
-    });
+    } else {
+        each([&](int b, unsigned long long key, int) {
+            if (ordered((float)score_of(b, key)) >= t) take(b, key);
+        });
+    }
     __syncthreads();
     int n = listed;
     if (n > CAP) {
@@ -475,7 +490,7 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
         };
         auto count_of = [&](auto belongs) -> int {
             int c = 0;
-            each([&](int b, unsigned long long key) { c += belongs(ordered64(score_of(b, key) + 0.0), flat_of(b, key)); });
+            each([&](int b, unsigned long long key, int) { c += belongs(ordered64(score_of(b, key) + 0.0), flat_of(b, key)); });
             return block_count(c, &cell);
         };
         // asked first: whether it is -inf (most words forbidden), or all are equals of the best (the next of two probes)
@@ -487,7 +502,7 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
             probe = lo + (hi - lo) / 2 + 1;
             if (best_next && lo < hi) {
                 unsigned long long most = 0;
-                each([&](int b, unsigned long long key) { most = max(most, ordered64(score_of(b, key) + 0.0)); });
+                each([&](int b, unsigned long long key, int) { most = max(most, ordered64(score_of(b, key) + 0.0)); });
                 const unsigned high = __reduce_max_sync(0xffffffffu, (unsigned)(most >> 32));
                 const unsigned low = __reduce_max_sync(0xffffffffu, (unsigned)(most >> 32) == high ? (unsigned)most : 0u);
                 __syncthreads();
@@ -508,7 +523,7 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
         __syncthreads();
         if (tid == 0) listed = 0;
         __syncthreads();
-        each([&](int b, unsigned long long key) {
+        each([&](int b, unsigned long long key, int) {
             const double s = score_of(b, key);
             const unsigned long long o = ordered64(s + 0.0);
             const long long f = flat_of(b, key);
@@ -571,11 +586,13 @@ RI_API int ri_beam_select(const float* logits, long long ld, int vocab, const fl
     RI_CHECKED((int)cudaGetDevice(&device));
     if (device > 63 || !(configured >> device & 1)) {
         RI_CHECKED((int)cudaFuncSetAttribute(beam_slices_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring));
+        RI_CHECKED((int)cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, KEPT * 4));
         if (device <= 63) configured |= 1ull << device;
     }
     RI_CHECKED(ri_launch(beam_slices_kernel, dim3(min(rows * slices, CTAS * sms)), dim3(ST), ring, s, logits, ld, vocab, scores, picks, rows * slices,
                          slices, a_slice, best, stat));
-    RI_CHECKED(ri_launch(beam_merge_kernel, dim3(groups), dim3(MT), 0, s, best, stat, scores, vocab, beams, slices, picks, out_scores, out_rows,
+    const int rounded = beams * slices * 2 * picks <= KEPT ? beams * slices * 2 * picks * 4 : 0;
+    RI_CHECKED(ri_launch(beam_merge_kernel, dim3(groups), dim3(MT), rounded, s, best, stat, scores, vocab, beams, slices, picks, out_scores, out_rows,
                          out_tokens));
     return ri_launch_status();
 }
