@@ -54,12 +54,11 @@ __device__ __forceinline__ void cp_async16(void* smem, const void* gmem, bool va
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N)); }
-__device__ __forceinline__ void ldmatrix_x4(unsigned (&r)[4], const void* p) {
-    const unsigned s = (unsigned)__cvta_generic_to_shared(p);
+// by 32-bit shared addresses: through pointers every fragment cost half a dozen instructions of address
+__device__ __forceinline__ void ldmatrix_x4(unsigned (&r)[4], unsigned s) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s));
 }
-__device__ __forceinline__ void ldmatrix_x4_trans(unsigned (&r)[4], const void* p) {
-    const unsigned s = (unsigned)__cvta_generic_to_shared(p);
+__device__ __forceinline__ void ldmatrix_x4_trans(unsigned (&r)[4], unsigned s) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s));
 }
@@ -161,6 +160,7 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
     constexpr int PIECES = (KT * CH + THREADS - 1) / THREADS;      // 16-byte pieces of a tile's keys a thread fetches
     constexpr int KROW = TMA ? HD : ROW;
     constexpr int STAGE = 2 * KT * KROW;                   // elements
+    constexpr int KROW_BYTES = TMA ? 128 : ROW * 2;        // by TMA: of a block of 64 columns
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.Hq / a.Hkv, splits = a.shared_splits + a.own_splits;
     bf16* KVs = reinterpret_cast<bf16*>(smem);             // [STAGES][K | V][KT][KROW]
@@ -168,6 +168,16 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
     uint64_t* full = reinterpret_cast<uint64_t*>(Qs + RTILES * 16 * ROW);
     const int rt = warp / KG, kg = warp % KG;
     const bool works = warp < RTILES * KG;
+    // where a lane's fragments lie in a stage, in bytes: a row of keys and one of values.  By TMA, columns 16 ks on are an exclusive or away
+    // (the swizzle's bits are the only ones below a row), 64 columns a block; else 32 bytes a step
+    const int k_row = kg * WK + (lane & 7) + (lane >> 4) * 8, v_row = kg * WK + (lane & 15);
+    const unsigned base = smem_u32(KVs), q_at = smem_u32(Qs) + ((rt * 16 + (lane & 15)) * ROW + (lane >> 4) * 8) * 2;
+    const unsigned k_at = k_row * KROW_BYTES + (TMA ? ((((lane >> 3) & 1) ^ (k_row & 7)) << 4) : ((lane >> 3) & 1) * 16);
+    const unsigned v_at = KT * KROW * 2 + v_row * KROW_BYTES + (TMA ? (((lane >> 4) ^ (v_row & 7)) << 4) : (lane >> 4) * 16);
+    auto step = [&](unsigned at, int ks) -> unsigned {     // 16 columns a step
+        if constexpr (TMA) return (at ^ ((ks & 3) << 5)) + (ks >> 2) * (KT * 128);
+        else return at + ks * 32;
+    };
 
     const int t0 = lo / KT, tiles = (hi + KT - 1) / KT - t0;
     const size_t head_step = (size_t)a.page_size * HD, value_step = (size_t)a.Hkv * head_step;
@@ -283,23 +293,20 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
         }
         if (t + STAGES - 1 < tiles) fetch(t + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
         if constexpr (!TMA) cp_async_commit();
-        bf16* Ks = KVs + stage * STAGE;
-        bf16* Vs = Ks + KT * KROW;
+        bf16* Vs = KVs + stage * STAGE + KT * KROW;
+        const unsigned stage_at = base + stage * (STAGE * 2);
         if (++stage == STAGES) { stage = 0; parity ^= 1u; }
         const int kw0 = kg * WK, key0 = (t0 + t) * KT + kw0;
         if (!works || key0 >= hi || key0 + WK <= lo) continue;
         const bool edge = key0 < lo || key0 + WK > hi;
-        // where the 16 bytes of columns col .. col + 7 of row `row` lie
-        auto at = [&](bf16* tile, int row, int col) -> bf16* {
-            if constexpr (TMA) return tile + (col >> 6) * (KT * 64) + row * 64 + ((((col & 63) >> 3) ^ (row & 7)) << 3);
-            else return tile + row * ROW + col;
-        };
         if constexpr (TMA) {
             if (edge) {
                 // values of keys outside meet a weight of zero, but what lies there may be no number
                 for (int i = lane; i < WK * CH; i += 32) {
                     const int r = i / CH, key = key0 + r;
-                    if (key < lo || key >= hi) *reinterpret_cast<uint4*>(at(Vs, kw0 + r, (i - r * CH) * 8)) = make_uint4(0u, 0u, 0u, 0u);
+                    const int col = (i - r * CH) * 8, row = kw0 + r;
+                    if (key < lo || key >= hi)
+                        *reinterpret_cast<uint4*>(Vs + (col >> 6) * (KT * 64) + row * 64 + ((((col & 63) >> 3) ^ (row & 7)) << 3)) = make_uint4(0u, 0u, 0u, 0u);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // ahead of the copy that the stage is used for next
                 __syncwarp();
@@ -311,11 +318,11 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             unsigned qf[4];                                // (from shared memory every tile: its registers make room for a second CTA)
-            ldmatrix_x4(qf, Qs + (rt * 16 + (lane & 15)) * ROW + ks * 16 + (lane >> 4) * 8);
+            ldmatrix_x4(qf, q_at + ks * 32);
 #pragma unroll
             for (int n2 = 0; n2 < NK / 2; ++n2) {
                 unsigned kf[4];
-                ldmatrix_x4(kf, at(Ks, kw0 + n2 * 16 + (lane & 7) + (lane >> 4) * 8, ks * 16 + ((lane >> 3) & 1) * 8));
+                ldmatrix_x4(kf, step(stage_at + k_at, ks) + n2 * 16 * KROW_BYTES);
                 mma_bf16(s[2 * n2], qf, kf[0], kf[1]);
                 mma_bf16(s[2 * n2 + 1], qf, kf[2], kf[3]);
             }
@@ -369,7 +376,7 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
 #pragma unroll
             for (int np = 0; np < NT / 2; ++np) {
                 unsigned vf[4];
-                ldmatrix_x4_trans(vf, at(Vs, kw0 + n2 * 16 + (lane & 15), np * 16 + (lane >> 4) * 8));
+                ldmatrix_x4_trans(vf, step(stage_at + v_at, np) + n2 * 16 * KROW_BYTES);
                 mma_bf16(o[2 * np], ph, vf[0], vf[1]);
                 mma_bf16(o[2 * np + 1], ph, vf[2], vf[3]);
                 mma_bf16(o[2 * np], pl, vf[0], vf[1]);
@@ -432,6 +439,8 @@ __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, i
     const int splits = a.shared_splits + a.own_splits;
     bf16* Ks = reinterpret_cast<bf16*>(smem) + warp * 2 * OWN_KEYS * ROW;
     bf16* Vs = Ks + OWN_KEYS * ROW;
+    const unsigned k_at = smem_u32(Ks) + (((lane & 7) + (lane >> 4) * 8) * ROW + ((lane >> 3) & 1) * 8) * 2;
+    const unsigned v_at = smem_u32(Vs) + ((lane & 15) * ROW + (lane >> 4) * 8) * 2;
     const int* bt = a.table + (size_t)r * a.table_stride;
     const size_t head_step = (size_t)a.page_size * HD, value_step = (size_t)a.Hkv * head_step;
     // a lane's half of a row, 16 rows, two lanes each; its page's number is read a step ahead
@@ -479,7 +488,7 @@ __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, i
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             unsigned kf[4];
-            ldmatrix_x4(kf, Ks + ((lane & 7) + (lane >> 4) * 8) * ROW + ks * 16 + ((lane >> 3) & 1) * 8);
+            ldmatrix_x4(kf, k_at + ks * 32);
             mma_8rows(s[0], qf[ks][0], qf[ks][1], kf[0], kf[1]);
             mma_8rows(s[1], qf[ks][0], qf[ks][1], kf[2], kf[3]);
         }
@@ -518,7 +527,7 @@ __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, i
 #pragma unroll
         for (int np = 0; np < NT / 2; ++np) {
             unsigned vf[4];
-            ldmatrix_x4_trans(vf, Vs + (lane & 15) * ROW + np * 16 + (lane >> 4) * 8);
+            ldmatrix_x4_trans(vf, v_at + np * 32);
             mma_8rows(o[2 * np], ph[0], ph[1], vf[0], vf[1]);
             mma_8rows(o[2 * np + 1], ph[0], ph[1], vf[2], vf[3]);
             mma_8rows(o[2 * np], pl[0], pl[1], vf[0], vf[1]);
@@ -542,15 +551,19 @@ __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, i
     }
 }
 
-// Tiles of shared keys a CTA takes: the fewest that leave all groups' ranges together no more CTAs than the `target` that run at once, and the
-// longest group no more ranges than there is room for
-__device__ __forceinline__ int tiles_a_range(const Args& a, int ctas_a_range, int KT) {
+// Which range of shared keys the `range`-th is: of group g, its `split`-th of n, `per` tiles long.  `per` is the least that leaves all groups
+// together no more than `ranges`, and the longest no more than there is room for; no range (n = 0) where the groups have fewer.
+struct Range {
+    int g, split, n, per;
+};
+__device__ __forceinline__ Range range_of(const Args& a, int range, int ranges, int KT) {
     const int lane = threadIdx.x & 31;
     auto tiles_of = [&](int g) {
+        if (g >= a.groups) return 0;
         const int n = keys_of(a, g * a.beams), lo = a.window > 0 ? max(0, n - a.window) : 0, hi = max(lo, min(a.shared_len[g], n));
         return hi > lo ? (hi + KT - 1) / KT - lo / KT : 0;
     };
-    const int first = lane < a.groups ? tiles_of(lane) : 0;        // (a group a lane is read once)
+    const int first = tiles_of(lane);                      // (of 32 groups or fewer, each is read once)
     int total = first, most = first;
     for (int g = lane + 32; g < a.groups; g += 32) {
         const int n = tiles_of(g);
@@ -559,7 +572,6 @@ __device__ __forceinline__ int tiles_a_range(const Args& a, int ctas_a_range, in
     }
     total = __reduce_add_sync(0xffffffffu, total);
     most = __reduce_max_sync(0xffffffffu, most);
-    const int ranges = max(1, a.target / ctas_a_range);
     int per = max(1, max((total + ranges - 1) / ranges, (most + a.shared_splits - 1) / a.shared_splits));
     while (per < most) {
         int n = (first + per - 1) / per;
@@ -567,39 +579,59 @@ __device__ __forceinline__ int tiles_a_range(const Args& a, int ctas_a_range, in
         if (__reduce_add_sync(0xffffffffu, n) <= ranges) break;
         per += (per >> 3) + 1;
     }
-    return per;
+    Range out{0, 0, 0, per};
+    for (int g0 = 0, before = 0; g0 < a.groups; g0 += 32) {
+        const int n = ((g0 ? tiles_of(g0 + lane) : first) + per - 1) / per;
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, before + upto > range);
+        if (here) {
+            const int l = __ffs(here) - 1;
+            out.g = g0 + l;
+            out.n = __shfl_sync(0xffffffffu, n, l);
+            out.split = range - (before + __shfl_sync(0xffffffffu, upto, l) - out.n);
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return out;
 }
 
-// Blocks: first (range of shared keys, group, key head, row chunk), then a warp for (range of the row's own keys, row, key head, eight heads).
+// Blocks: first (range of shared keys, key head, row chunk), then a warp for (range of the row's own keys, row, key head, eight heads).
 template <int RTILES, bool TMA>
 __global__ void __launch_bounds__(THREADS, CTAS)
-beams_kernel(const __grid_constant__ CUtensorMap map, Args a, int chunks, int own_chunks) {
+beams_kernel(const __grid_constant__ CUtensorMap map, Args a, int ranges, int chunks, int own_chunks) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     pdl_wait();
     pdl_trigger();
     constexpr int KT = tile_keys<RTILES>();
-    const int G = a.Hq / a.Hkv;
+    const int G = a.Hq / a.Hkv, splits = a.shared_splits + a.own_splits;
     int id = blockIdx.x, from, to;
-    const int n_shared = a.groups * a.Hkv * chunks * a.shared_splits;
+    const int n_shared = ranges * a.Hkv * chunks;
     if (id < n_shared) {
         const int chunk = id % chunks;        id /= chunks;
-        const int kvh = id % a.Hkv;           id /= a.Hkv;
-        const int g = id % a.groups, split = id / a.groups;
-        shared_range(a, g, from, to);
-        const int per = tiles_a_range(a, a.Hkv * chunks, KT);
+        const int kvh = id % a.Hkv;
+        const Range x = range_of(a, id / a.Hkv, ranges, KT);
+        if (x.n == 0) return;
+        shared_range(a, x.g, from, to);                    // (none where the rows do not share what they are said to)
         // ranges start at multiples of the tiles' size
-        const int lo = split == 0 ? from : (int)min((long long)to, ((long long)(from / KT) + (long long)split * per) * KT);
-        const int hi = (int)min((long long)to, ((long long)(from / KT) + (long long)(split + 1) * per) * KT);
+        const int lo = x.split == 0 ? from : (int)min((long long)to, ((long long)(from / KT) + (long long)x.split * x.per) * KT);
+        const int hi = (int)min((long long)to, ((long long)(from / KT) + (long long)(x.split + 1) * x.per) * KT);
         const int m0 = chunk * RTILES * 16, m_count = min(RTILES * 16, a.beams * G - m0);
-        if (lo >= hi) {                                    // the range is empty: that is all there is to say
-            for (int r = threadIdx.x; r < m_count; r += THREADS) {
-                const int b = (m0 + r) / G, h = m0 + r - b * G;
-                a.part_lse[((size_t)(g * a.beams + b) * a.Hq + kvh * G + h) * (a.shared_splits + a.own_splits) + split] = -INFINITY;
-            }
-            return;
+        // the last one says of the ranges that the group does not have that they are empty
+        const int empty_from = lo >= hi ? x.split : x.split + 1, empty_to = x.split + 1 == x.n ? a.shared_splits : x.split + 1;
+        for (int r = threadIdx.x; r < m_count && empty_from < empty_to; r += THREADS) {
+            const int b = (m0 + r) / G, h = m0 + r - b * G;
+            for (int s = empty_from; s < empty_to; ++s)
+                a.part_lse[((size_t)(x.g * a.beams + b) * a.Hq + kvh * G + h) * splits + s] = -INFINITY;
         }
-        attend<RTILES, TMA>(a, &map, smem, g, kvh, m0, m_count, a.table + (size_t)g * a.beams * a.table_stride, lo, hi, split);
+        if (lo < hi)
+            attend<RTILES, TMA>(a, &map, smem, x.g, kvh, m0, m_count, a.table + (size_t)x.g * a.beams * a.table_stride, lo, hi, x.split);
         return;
     }
     id = (id - n_shared) * WARPS + (threadIdx.x >> 5);
@@ -607,12 +639,20 @@ beams_kernel(const __grid_constant__ CUtensorMap map, Args a, int chunks, int ow
     const int kvh = id % a.Hkv;           id /= a.Hkv;
     const int split = id % a.own_splits, r = id / a.own_splits;
     if (r >= a.groups * a.beams) return;
-    shared_range(a, r / a.beams, from, to);
+    const int g = r / a.beams, heads = min(8, G - chunk * 8), lane = threadIdx.x & 31;
+    shared_range(a, g, from, to);
     const int end = keys_of(a, r);
     const int begin = to > from ? to : (a.window > 0 ? max(0, end - a.window) : 0);
+    if (split == 0) {
+        // a group without a tile of shared keys has no CTA that says so
+        const int n = keys_of(a, g * a.beams), lo = a.window > 0 ? max(0, n - a.window) : 0;
+        if (min(a.shared_len[g], n) <= lo)
+            for (int i = lane; i < heads * a.shared_splits; i += 32)
+                a.part_lse[((size_t)r * a.Hq + kvh * G + chunk * 8 + i / a.shared_splits) * splits + i % a.shared_splits] = -INFINITY;
+    }
     const int steps = (max(0, end - begin) + OWN_KEYS - 1) / OWN_KEYS, per = (steps + a.own_splits - 1) / a.own_splits;
     const int lo = (int)min((long long)end, begin + (long long)split * per * OWN_KEYS), hi = min(end, lo + per * OWN_KEYS);
-    attend_own(a, smem, r, kvh, kvh * G + chunk * 8, min(8, G - chunk * 8), lo, hi, a.shared_splits + split);
+    attend_own(a, smem, r, kvh, kvh * G + chunk * 8, heads, lo, hi, a.shared_splits + split);
 }
 
 // out[r, h, :] = sum over ranges of 2^(lse - max) part / sum of 2^(lse - max); a row without keys: zeros.  A warp a head: a lane knows one
@@ -713,9 +753,11 @@ int run(Args a, long long pages, cudaStream_t stream) {
     }
     const int G = a.Hq / a.Hkv, chunks = (a.beams * G + RTILES * 16 - 1) / (RTILES * 16), own_chunks = (G + 7) / 8;
     const long long units = (long long)a.groups * a.beams * a.Hkv * own_chunks * a.own_splits;
-    const long long blocks = (long long)a.groups * a.Hkv * chunks * a.shared_splits + (units + WARPS - 1) / WARPS;
+    // ranges of shared keys: as many as make `target` CTAs, and one a group at least
+    const int made = a.target / (a.Hkv * chunks), ranges = made > a.groups ? made : a.groups;
+    const long long blocks = (long long)ranges * a.Hkv * chunks + (units + WARPS - 1) / WARPS;
     if (blocks * WARPS > 0x7fffffffll) return (int)cudaErrorInvalidValue;
-    return ri_launch(beams_kernel<RTILES, TMA>, dim3((unsigned)blocks), dim3(THREADS), (size_t)bytes, stream, map, a, chunks, own_chunks);
+    return ri_launch(beams_kernel<RTILES, TMA>, dim3((unsigned)blocks), dim3(THREADS), (size_t)bytes, stream, map, a, ranges, chunks, own_chunks);
 }
 bool by_tma(const void* cache, int page_size, long long pages, int Hkv) {
     return BY_TMA && (page_size == 8 || page_size == 16 || page_size == 32 || page_size % 64 == 0) && (reinterpret_cast<uintptr_t>(cache) & 15) == 0 &&

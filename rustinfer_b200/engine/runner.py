@@ -162,7 +162,7 @@ class _DecodeGraph:
             num_tokens=bucket, num_entries=bucket, token_ids=v[0], positions=v[1], cu_q=v[2], kv_len=v[3],
             state_slots=v[4], groups=gsteps, entries=[], max_q_len=1,
             max_kv_len=runner.max_model_len, decode_only=True, indices=indices,
-            beams=beams, shared_len=v[-1] if beams > 1 else None, max_own_len=min(256, runner.max_model_len) if beams > 1 else 0)
+            beams=beams, shared_len=v[-1] if beams > 1 else None, max_own_len=min(64, runner.max_model_len) if beams > 1 else 0)
         self.rows = v[5]
         # one eager run (libraries pick their algorithms, lazy kernels get built), then capture
         torch.cuda.synchronize()
@@ -236,10 +236,9 @@ class _DecodeGraph:
                     raise StepError("a token would be written to a page that was given back")
                 self.h_slot_of_token[gi][i] = page * ps + pos % ps
         if self.h_shared is not None:
-            k = self.beams
-            for j in range(self.bucket // k):
-                rows = [e.request_id for e in entries[j * k: (j + 1) * k]]
-                self.h_shared[j] = cache.common_length(rows) if len(rows) == k else 0
+            common = runner._common(entries, self.beams)
+            self.h_shared[: len(common)] = common
+            self.h_shared[len(common):] = 0
         for i in range(len(entries), self.bucket):           # padding rows
             if self.row_owner[i] is not None:
                 self.row_owner[i] = None
@@ -266,6 +265,11 @@ class _DecodeGraph:
 
 class ModelRunner:
     """Model, cache and step function of one model folder on one GPU."""
+
+    # Steps of beams read their requests' common keys once when all beams together see at least so many of them: below, the rows' own
+    # kernel, whose later rows find them in L2, is sooner (us a layer of 8 key heads of 64, rows / beams: 64 rows behind 300 keys 9 / 15,
+    # behind 1,000 18 / 16, behind 4,000 61 / 28; 8 rows behind 4,000 14 / 16)
+    beam_keys = 64 * 1024
 
     def __init__(self, model_dir: str, dtype="bfloat16", device="cuda:0", max_model_len: int = 4096,
                  page_size: int = 16, num_pages: Optional[int] = None, max_batch_seqs: int = 64,
@@ -462,6 +466,10 @@ class ModelRunner:
         return n
 
     # --------------------------------------------------------------------------- plan
+    def _common(self, entries: Sequence[StepEntry], beams: int) -> List[int]:
+        """Keys that the requests of every `beams` entries have in common."""
+        return [self.cache.common_length([e.request_id for e in entries[i: i + beams]]) for i in range(0, len(entries), beams)]
+
     def _validate(self, entries: Sequence[StepEntry]) -> Optional[np.ndarray]:
         """Raises `StepError` for a step that cannot be; returns the ids of a step of many tokens as one array (None: as they are)."""
         if not entries:
@@ -537,7 +545,7 @@ class ModelRunner:
         sections.append(np.asarray(row_slots, dtype=np.int64))
         shared = None
         if beams > 1:
-            shared = np.asarray([self.cache.common_length([e.request_id for e in entries[i: i + beams]]) for i in range(0, B, beams)], dtype=np.int64)
+            shared = np.asarray(self._common(entries, beams), dtype=np.int64)
             sections.append(shared)
         shape = StepShape(q_lens, pos0, cu_q, kv_len, slots)
         built = [(need, need.build(shape)) for need in self.index_needs]
@@ -588,10 +596,12 @@ class ModelRunner:
         that the next step overwrites (for callers that consume it at once).
 
         `beams` above 1: the entries are single tokens, and every `beams` of them that follow one another are forks of
-        one request (`fork`), whose common keys are read once."""
+        one request (`fork`), whose common keys are read once where there are many (`beam_keys`)."""
         ids = self._validate(entries)
         if beams > 1 and (len(entries) % beams or any(len(e.tokens) != 1 for e in entries)):
             raise StepError(f"{len(entries)} entries are no single tokens of {beams} beams a request")
+        if beams > 1 and beams * sum(self._common(entries, beams)) < self.beam_keys:
+            beams = 0
         lease = self.cache.lease([(e.request_id, len(e.tokens)) for e in entries])
         try:
             self._zero_new_state()

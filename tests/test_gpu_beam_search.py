@@ -44,7 +44,9 @@ def _engine(folder, dtype, **kw):
     from rustinfer_b200.engine.engine import Engine
     args = dict(max_batch_seqs=12, max_model_len=128, paged_block_size=8, num_blocks=200, max_batch_tokens=128, capture_sizes=[])
     args.update(kw)
-    return Engine(folder, dtype=dtype, **args)
+    eng = Engine(folder, dtype=dtype, **args)
+    eng.runner.beam_keys = 0                               # however few keys they share, beams read them together
+    return eng
 
 
 def _log_probs(runner, prompt):
@@ -149,6 +151,7 @@ def test_forks_and_reorders_of_requests(folder, family, name, sizes):
     from rustinfer_b200.engine.runner import ModelRunner, StepEntry
     r = ModelRunner(folder(family, name), dtype="float32", max_model_len=128, page_size=8, num_pages=80, max_batch_seqs=6, max_batch_tokens=128,
                     capture_sizes=sizes)
+    r.beam_keys = 0
     vocab = r.spec.vocab_size
     held = {"a": random_ids(21, vocab, 1)}
     r.open("z")                                            # a neighbour, so that pages and slots lie apart
@@ -193,6 +196,17 @@ def test_forks_and_reorders_of_requests(folder, family, name, sizes):
     for i in order:
         r.close(i)
     assert r.cache.free_pages() == {g: 80 for g in r.layout.paged_groups()}
+
+
+def test_few_common_keys_are_read_row_by_row(folder):
+    """Below `beam_keys` a step of beams is a step of rows; from there on one of beams."""
+    from rustinfer_b200.engine.beam import BeamParams
+    eng = _engine(folder("llama", "D"), "bfloat16", capture_sizes=[4])
+    r, prompt = eng.runner, random_ids(40, 1000, 3)
+    for keys, graphs in ((4 * 40 + 1, [4]), (4 * 40, [4, (4, 4)])):
+        r.beam_keys = keys
+        eng.beam_search([prompt], BeamParams(beams=4, max_tokens=4, ignore_eos=True))
+        assert sorted(r._graphs, key=str) == sorted(graphs, key=str)
 
 
 def test_requests_that_follow_a_search(folder):
