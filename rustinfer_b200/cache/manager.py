@@ -284,7 +284,9 @@ class CacheManager:
                 mine, theirs = r.tables[g], reqs[p].tables[g]
                 if mine is theirs:
                     continue
-                at = next((b for b, (x, y) in enumerate(zip(mine[:full], theirs[:full])) if x != y), full)
+                # pages of tokens that two members have in common are one page: looked at from there on
+                b0 = min(r.common, reqs[p].common, reqs[0].length) // self.page_size
+                at = next((b for b in range(b0, full) if mine[b] != theirs[b]), full)
                 if at < full:
                     fresh.append((r, at, theirs[at:full]))
             for _r, _at, pages in fresh:                   # everyone's new pages before anyone's old ones are given back
