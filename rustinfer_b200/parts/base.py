@@ -194,13 +194,13 @@ class StepContext:
     max_q_len: int
     max_kv_len: int                     # an upper bound of kv_len (exact in eager steps)
     decode_only: bool
+    # what the model's parts declared through `step_indices()`: key -> tuple of device tensors
+    indices: Dict[Hashable, Tuple[torch.Tensor, ...]] = field(default_factory=dict)
     # steps of single tokens whose entries are beams: entries per request, keys at the start that a request's entries
     # share [entries / beams], and about how many keys the longest rest has (0: entries have nothing to do with one another)
     beams: int = 0
     shared_len: Optional[torch.Tensor] = None
     max_own_len: int = 0
-    # what the model's parts declared through `step_indices()`: key -> tuple of device tensors
-    indices: Dict[Hashable, Tuple[torch.Tensor, ...]] = field(default_factory=dict)
 
     def index(self, need: "StepIndex") -> Tuple[torch.Tensor, ...]:
         try:
