@@ -32,20 +32,21 @@ constexpr int OROW = HD + 8;                               // rows of outputs in
 constexpr int CH = HD / 8;                                 // 16-byte pieces a row
 constexpr int KS = HD / 16;
 constexpr int NT = HD / 8;
-constexpr int WARPS = 8;
+constexpr int WARPS = 4;
 constexpr int THREADS = 32 * WARPS;
-constexpr int CTAS = HD <= 128 ? 2 : 1;                    // CTAs an SM that registers and shared memory are cut for
+constexpr int CTAS = HD <= 64 ? 4 : HD <= 128 ? 2 : 1;     // CTAs an SM that registers and shared memory are cut for
 constexpr int MAX_BEAMS = 64;
 constexpr int OWN_KEYS = 16;                               // keys of its own a row's warp takes at a time
 constexpr bool BY_TMA = HD == 64 || HD == 128;
 constexpr int TKB = HD / 64;                               // 64-column blocks of a head
 constexpr unsigned SPIN_LIMIT = 1u << 20;
 
-// Keys of a tile: 32 a warp where a CTA has room for two or three of them
-template <int RTILES> constexpr int tile_keys() { return HD <= 64 && RTILES <= 2 ? 128 : 64; }
-constexpr int STAGES = HD <= 64 ? 3 : 2;
+constexpr int KT = 64;                                     // keys of a tile
+constexpr int STAGES = 2;
+// (8 x 8 beams, heads of 64, us behind 4,096 / 16,384 keys: 4 warps, 4 CTAs an SM 28 / 69; 8 warps, 2 CTAs, tiles of 128, 3 stages 28 / 79;
+// 4 warps and 3 CTAs 32 / 83, 5 CTAs 31 / 76.  Heads of 128, 4 x 16 beams behind 12,000: 4 warps, 2 CTAs 84; 8 warps, 2 CTAs 89)
 // rows of shared keys are split over RTILES warps, a tile's keys over the others
-template <int RTILES> constexpr int key_groups() { return WARPS / RTILES < tile_keys<RTILES>() / 16 ? WARPS / RTILES : tile_keys<RTILES>() / 16; }
+template <int RTILES> constexpr int key_groups() { return WARPS / RTILES < KT / 16 ? WARPS / RTILES : KT / 16; }
 
 __device__ __forceinline__ void cp_async16(void* smem, const void* gmem, bool valid) {
     const unsigned s = (unsigned)__cvta_generic_to_shared(smem);
@@ -154,7 +155,7 @@ __device__ __forceinline__ void shared_range(const Args& a, int g, int& from, in
 template <int RTILES, bool TMA>
 __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, unsigned char* smem, int g, int kvh, int m0, int m_count, const int* bt,
                                        int lo, int hi, int part) {
-    constexpr int KT = tile_keys<RTILES>(), KG = key_groups<RTILES>();
+    constexpr int KG = key_groups<RTILES>();
     constexpr int WK = KT / KG;                            // keys a warp takes of a tile
     constexpr int NK = WK / 8;
     constexpr int PIECES = (KT * CH + THREADS - 1) / THREADS;      // 16-byte pieces of a tile's keys a thread fetches
@@ -556,7 +557,7 @@ __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, i
 struct Range {
     int g, split, n, per;
 };
-__device__ __forceinline__ Range range_of(const Args& a, int range, int ranges, int KT) {
+__device__ __forceinline__ Range range_of(const Args& a, int range, int ranges) {
     const int lane = threadIdx.x & 31;
     auto tiles_of = [&](int g) {
         if (g >= a.groups) return 0;
@@ -609,14 +610,13 @@ beams_kernel(const __grid_constant__ CUtensorMap map, Args a, int ranges, int ch
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     pdl_wait();
     pdl_trigger();
-    constexpr int KT = tile_keys<RTILES>();
     const int G = a.Hq / a.Hkv, splits = a.shared_splits + a.own_splits;
     int id = blockIdx.x, from, to;
     const int n_shared = ranges * a.Hkv * chunks;
     if (id < n_shared) {
         const int chunk = id % chunks;        id /= chunks;
         const int kvh = id % a.Hkv;
-        const Range x = range_of(a, id / a.Hkv, ranges, KT);
+        const Range x = range_of(a, id / a.Hkv, ranges);
         if (x.n == 0) return;
         shared_range(a, x.g, from, to);                    // (none where the rows do not share what they are said to)
         // ranges start at multiples of the tiles' size
@@ -706,7 +706,7 @@ beams_join_kernel(const float* part_o, const float* part_lse, bf16* out, int out
 
 template <int RTILES, bool TMA>
 constexpr size_t smem_bytes() {
-    const size_t kv = (size_t)STAGES * 2 * tile_keys<RTILES>() * (TMA ? HD : ROW) * sizeof(bf16) + (size_t)RTILES * 16 * ROW * sizeof(bf16) + 64;
+    const size_t kv = (size_t)STAGES * 2 * KT * (TMA ? HD : ROW) * sizeof(bf16) + (size_t)RTILES * 16 * ROW * sizeof(bf16) + 64;
     const size_t merge = (WARPS * 16 * (size_t)OROW + 2 * WARPS * 16) * sizeof(float), own = (size_t)WARPS * 2 * OWN_KEYS * ROW * sizeof(bf16);
     return 1024 /*alignment*/ + (kv > merge ? (kv > own ? kv : own) : (merge > own ? merge : own));
 }
@@ -748,7 +748,7 @@ int run(Args a, long long pages, cudaStream_t stream) {
     }
     CUtensorMap map = {};
     if constexpr (TMA) {
-        a.box_rows = a.page_size < tile_keys<RTILES>() ? a.page_size : tile_keys<RTILES>() == 128 && a.page_size % 128 ? 64 : tile_keys<RTILES>();
+        a.box_rows = a.page_size < KT ? a.page_size : KT;
         RI_CHECKED(cache_map(a.cache, pages * 2 * a.Hkv * a.page_size, a.box_rows, &map));
     }
     const int G = a.Hq / a.Hkv, chunks = (a.beams * G + RTILES * 16 - 1) / (RTILES * 16), own_chunks = (G + 7) / 8;

@@ -2165,7 +2165,7 @@ def _attention_beams_plan(rows: int, beams: int, num_heads: int, num_kv_heads: i
     lib = L.attention_beams(head_dim)
     shared, own = attention_beams_splits(most_shared, most_own)
     at_once = int(lib.ri_attention_beams_ctas_per_sm()) * num_sms
-    own_ctas = -(-rows * num_kv_heads * -(-(num_heads // num_kv_heads) // 8) * own // 8)
+    own_ctas = -(-rows * num_kv_heads * -(-(num_heads // num_kv_heads) // 8) * own // 4)
     return (lib.ri_attention_beams, shared, own, at_once - min(at_once // 4, own_ctas // 4), *decode_scratch_floats(rows, num_heads, head_dim, shared + own))
 
 
