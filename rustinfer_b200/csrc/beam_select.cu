@@ -92,11 +92,11 @@ __device__ __forceinline__ unsigned reach(unsigned mine, unsigned floor, unsigne
     return lo;
 }
 
-__device__ __forceinline__ void copy_async16(void* to, const void* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+__device__ __forceinline__ void copy_async16(unsigned to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to), "l"(from) : "memory");
 }
-__device__ __forceinline__ void copy_async4(void* to, const void* from) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+__device__ __forceinline__ void copy_async4(unsigned to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(to), "l"(from) : "memory");
 }
 
 __global__ void __launch_bounds__(ST, CTAS)
@@ -130,23 +130,35 @@ beam_slices_kernel(const float* logits, long long ld, int vocab, const float* sc
     };
     // A vector of the ring holds 16 aligned bytes: where the row starts `shift` elements behind a boundary, a thread's four elements lie in
     // its own and in the next lane's, and the warp fetches a 33rd.
+    const unsigned mine_at = (unsigned)__cvta_generic_to_shared(ring) + (warp * 33 + lane) * 16;
+    constexpr unsigned STEP = W * 33 * 16, STAGE = NV * STEP;      // bytes from a thread's vector to its next, and to the next stage
     auto fetch = [&](const Slice& s, int v, int stage) {
+        const int e0 = 4 * v - s.shift;                    // the chunk's first element
         if (v < s.v1 && !s.dead) {
+            const unsigned to = mine_at + stage * STAGE;
+            if (e0 >= 0 && e0 + 4 * CHUNK + 4 <= s.e_hi) { // all of it lies in the slice
+                const float* from = s.row + e0 + 4 * tid;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                float4* const to = ring + ((stage * NV + i) * W + warp) * 33;
-                const int first = v + i * ST + warp * 32;
-                for (int j = lane; j < 32 + (s.shift != 0); j += 32) {
-                    const int e = 4 * (first + j) - s.shift;
-                    if (e >= 0 && e + 4 <= s.e_hi) {
-                        copy_async16(to + j, s.row + e);
-                    } else {
+                for (int i = 0; i < NV; ++i) copy_async16(to + i * STEP, from + i * (4 * ST));
+                if (s.shift && lane == 0) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (e + k >= 0 && e + k < s.e_hi) copy_async4(reinterpret_cast<float*>(to + j) + k, s.row + e + k);
-                            else reinterpret_cast<float*>(to + j)[k] = -INFINITY;
-                    }
+                    for (int i = 0; i < NV; ++i) copy_async16(to + i * STEP + 32 * 16, from + i * (4 * ST) + 4 * 32);
                 }
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < NV; ++i)
+#pragma unroll 1
+                    for (int j = lane; j < 32 + (s.shift != 0); j += 32) {
+                        const int e = e0 + 4 * (i * ST + warp * 32 + j);
+                        const unsigned at = to + i * STEP + (j - lane) * 16;
+                        if (e >= 0 && e + 4 <= s.e_hi) {
+                            copy_async16(at, s.row + e);
+                        } else {
+                            for (int k = 0; k < 4; ++k)
+                                if (e + k >= 0 && e + k < s.e_hi) copy_async4(at + 4 * k, s.row + e + k);
+                                else asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 4 * k), "f"(-INFINITY) : "memory");
+                        }
+                    }
             }
         }
         asm volatile("cp.async.commit_group;\n" ::: "memory");
@@ -260,33 +272,42 @@ beam_slices_kernel(const float* logits, long long ld, int vocab, const float* sc
     if (v1 - v0 <= CHUNK) {
         if (own >= t) gather(x, v0);
     } else {
-        // the few chunks of a thread in which something reaches t are read once more, a thread an element
+        // the few chunks of a thread in which something reaches t are read once more, a thread a vector
         for (int c = 0, v = v0; v < v1; ++c, v += CHUNK)
             if (chunk_top[c][tid] >= tf) again[atomicAdd(&cell, 1)] = (unsigned short)(c * ST + tid);
         __syncthreads();
-        const int elements = cell * (4 * NV);
-        constexpr int AT_ONCE = 8;                         // loads in flight together
-        for (int i0 = tid; i0 < elements; i0 += AT_ONCE * ST) {
-            float again_x[AT_ONCE];
-            int again_e[AT_ONCE];
+        const int vectors = cell * NV;
+        constexpr int AT_ONCE = 2;                         // vectors in flight together
+        for (int i0 = tid; i0 < vectors; i0 += AT_ONCE * ST) {
+            float y[AT_ONCE][4];
+            int e[AT_ONCE];
 #pragma unroll
             for (int q = 0; q < AT_ONCE; ++q) {
                 const int i = i0 + q * ST;
-                again_e[q] = e_hi;
-                if (i < elements) {
-                    const int at = again[i / (4 * NV)], c = at / ST, j = i & (4 * NV - 1);
-                    again_e[q] = 4 * (v0 + c * CHUNK + (j >> 2) * ST + (at & (ST - 1))) + (j & 3);
+                e[q] = e_hi;
+                if (i < vectors) {
+                    const int at = again[i / NV], c = at / ST;
+                    e[q] = 4 * (v0 + c * CHUNK + (i & (NV - 1)) * ST + (at & (ST - 1)));
                 }
-                again_x[q] = again_e[q] < e_hi ? row[again_e[q]] : 0.f;
+                if (now.shift == 0 && e[q] + 4 <= e_hi) {
+                    const float4 f = *reinterpret_cast<const float4*>(row + e[q]);
+                    y[q][0] = f.x; y[q][1] = f.y; y[q][2] = f.z; y[q][3] = f.w;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[q][k] = e[q] + k < e_hi ? row[e[q] + k] : -INFINITY;
+                }
             }
 #pragma unroll
-            for (int q = 0; q < AT_ONCE; ++q) {
-                const unsigned o = key_of(fmaxf(again_x[q], -INFINITY));
-                if (again_e[q] < e_hi && o >= t) {
-                    const int to = atomicAdd(&listed, 1);
-                    if (to < CAP) list[to] = ((unsigned long long)o << 32) | (unsigned)(0xffffffffu - (unsigned)again_e[q]);
-                }
-            }
+            for (int q = 0; q < AT_ONCE; ++q)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (!(y[q][k] < tf)) {
+                        const unsigned o = key_of(fmaxf(y[q][k], -INFINITY));
+                        if (o >= t && e[q] + k < e_hi) {
+                            const int to = atomicAdd(&listed, 1);
+                            if (to < CAP) list[to] = ((unsigned long long)o << 32) | (unsigned)(0xffffffffu - (unsigned)(e[q] + k));
+                        }
+                    }
         }
     }
 
