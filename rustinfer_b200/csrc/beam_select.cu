@@ -26,12 +26,14 @@
 namespace {
 constexpr int ST = 256;                                    // threads of a slice
 constexpr int NV = 4;                                      // 16-byte loads of a thread a chunk
-constexpr int CTAS = 3;                                    // CTAs an SM, which walk over slices
-constexpr int STAGES = 3;                                  // chunks of a slice in flight
+constexpr int CTAS = 4;                                    // CTAs an SM, which walk over slices
+constexpr int STAGES = 2;                                  // chunks of a slice in shared memory
+// (512 rows of 128,256 logits, 48 picks of 16 beams, us a call: 4 CTAs and 2 stages 69, 3 and 3 73, 3 and 2 70; 512 threads, 2 and 2 73; chunks of
+// half the size 81.  The logits' stream with its sums alone takes 48)
 constexpr int MAX_CHUNKS = 8;                              // chunks of a slice
 constexpr int LISTS = 1024;                                // slices of a group whose sums are kept in shared memory
 constexpr int KEPT = 16384;                                // ... and elements of the pool whose rounded scores are
-constexpr int MT = 512;                                   // threads of a group
+constexpr int MT = 512;                                    // threads of a group
 constexpr int CAP = 1024;                                  // room of the gathering
 constexpr int MAX_PICKS = 128, MAX_BEAMS = 64;
 
