@@ -39,6 +39,7 @@ constexpr int MAX_BEAMS = 64;
 constexpr int OWN_KEYS = 16;                               // keys of its own a row's warp takes at a time
 constexpr bool BY_TMA = HD == 64 || HD == 128;
 constexpr int TKB = HD / 64;                               // 64-column blocks of a head
+constexpr int NO_KEY = (int)0x80000000;                    // in place of a page
 constexpr unsigned SPIN_LIMIT = 1u << 20;
 
 constexpr int KT = 64;                                     // keys of a tile
@@ -119,6 +120,7 @@ struct Args {
     const bf16* cache;
     const int* table;
     int table_stride, table_keys;                         // keys a row of the table has pages for
+    int pages;                                             // of the cache: a number outside stands for a page of zeros
     const int* kv_len;
     const int* shared_len;
     int beams, Hq, Hkv, page_size;
@@ -191,8 +193,9 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
             const int c = tid + i * THREADS, kk = c / CH, ch = c - kk * CH, key = (t0 + t) * KT + kk;
             from[i] = nullptr;
             if (c < KT * CH && key >= lo && key < hi) {
-                const int blk = shift >= 0 ? key >> shift : key / a.page_size;
-                from[i] = a.cache + ((size_t)bt[blk] * 2 * a.Hkv + kvh) * head_step + (size_t)(key - blk * a.page_size) * HD + ch * 8;
+                const int blk = shift >= 0 ? key >> shift : key / a.page_size, page = bt[blk];
+                if ((unsigned)page < (unsigned)a.pages)
+                    from[i] = a.cache + ((size_t)page * 2 * a.Hkv + kvh) * head_step + (size_t)(key - blk * a.page_size) * HD + ch * 8;
             }
         }
     };
@@ -200,12 +203,12 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
     const int boxes = KT / a.box_rows;                     // of keys, of 64 columns
     constexpr int MOST_BOXES = 2 * (KT / 8) * (BY_TMA ? TKB : 1);
     constexpr int TURNS = (MOST_BOXES + 31) / 32;          // (pages of 8 keys: more boxes than lanes)
-    int page_of[TURNS];                                    // (as it was read: nothing waits for the load before the fetch does)
+    int page_of[TURNS];                                    // (nothing waits for the load before the fetch does)
     auto look_up_boxes = [&](int t) {
 #pragma unroll
         for (int i = 0; i < TURNS; ++i) {
             const int box = lane + 32 * i, kv = box / (boxes * TKB), c = (box - kv * boxes * TKB) / TKB, key = (t0 + t) * KT + c * a.box_rows;
-            page_of[i] = -1;                               // boxes without a key in [lo, hi) are not fetched
+            page_of[i] = NO_KEY;                           // boxes without a key in [lo, hi) are not fetched
             if (box < 2 * boxes * TKB && key < hi && key + a.box_rows > lo) page_of[i] = bt[key / a.page_size];
         }
     };
@@ -214,7 +217,10 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
             if (warp == 0) {
                 int mine = 0;
 #pragma unroll
-                for (int i = 0; i < TURNS; ++i) mine += page_of[i] >= 0;
+                for (int i = 0; i < TURNS; ++i) {
+                    if (page_of[i] != NO_KEY && (unsigned)page_of[i] > (unsigned)a.pages) page_of[i] = a.pages;
+                    mine += page_of[i] != NO_KEY;
+                }
                 const int all = __reduce_add_sync(0xffffffffu, mine);
                 if (lane == 0) bar_expect(&full[stage], (unsigned)all * a.box_rows * 128);
                 __syncwarp();
@@ -222,9 +228,10 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
                 for (int i = 0; i < TURNS; ++i) {
                     const int box = lane + 32 * i, kv = box / (boxes * TKB), rest = box - kv * boxes * TKB, c = rest / TKB, kb = rest - c * TKB;
                     const int key = (t0 + t) * KT + c * a.box_rows;
-                    if (page_of[i] >= 0)
+                    if (page_of[i] != NO_KEY)
                         tma_load_2d(reinterpret_cast<unsigned char*>(KVs + stage * STAGE) + ((kv * TKB + kb) * KT + c * a.box_rows) * 128, map,
                                     &full[stage], kb * 64, ((page_of[i] * 2 + kv) * a.Hkv + kvh) * a.page_size + key % a.page_size);
+                    // (a page outside the cache: rows behind the matrix, which are read as zeros)
                 }
                 if (t + 1 < tiles) look_up_boxes(t + 1);
             }
@@ -451,7 +458,7 @@ __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, i
     };
     auto fetch = [&](bf16* to, int k0, int page, size_t step) {
         const int kk = lane >> 1;
-        const bool there = k0 + kk < hi;
+        const bool there = k0 + kk < hi && (unsigned)page < (unsigned)a.pages;
         const bf16* src = there ? a.cache + ((size_t)page * 2 * a.Hkv + kvh) * head_step + (size_t)((k0 + kk) % a.page_size) * HD + step : a.cache;
 #pragma unroll
         for (int ch = 0; ch < CH / 2; ++ch) {
@@ -761,7 +768,7 @@ int run(Args a, long long pages, cudaStream_t stream) {
 }
 bool by_tma(const void* cache, int page_size, long long pages, int Hkv) {
     return BY_TMA && (page_size == 8 || page_size == 16 || page_size == 32 || page_size % 64 == 0) && (reinterpret_cast<uintptr_t>(cache) & 15) == 0 &&
-           pages * 2 * Hkv * page_size < (1ll << 31);     // rows are 32-bit coordinates
+           (pages + 1) * 2 * Hkv * page_size < (1ll << 31);     // rows are 32-bit coordinates
 }
 template <bool TMA>
 int run_rows(const Args& a, long long pages, cudaStream_t s) {
@@ -784,7 +791,7 @@ RI_API int ri_attention_beams(const void* q, int q_stride, void* out, int out_st
         shared_splits + own_splits > 32 || !part_o || !part_lse || !error || (long long)groups * beams * Hq > 0x7fffffffll)
         return (int)cudaErrorInvalidValue;
     const Args a{(const bf16*)q, q_stride, (const bf16*)cache, table, table_stride, (int)min((long long)table_cols * page_size, 0x7fffffffll - 256),
-                 kv_len, shared_len, beams, Hq, Hkv, page_size, scale * 1.4426950408889634f, window, groups, shared_splits, own_splits,
+                 (int)min(pages, 0x7fffffffll), kv_len, shared_len, beams, Hq, Hkv, page_size, scale * 1.4426950408889634f, window, groups, shared_splits, own_splits,
                  target < 1 ? 1 : target, part_o, part_lse, error, 8};
     cudaStream_t s = (cudaStream_t)stream;
     bool tma = false;

@@ -138,7 +138,7 @@ beam_slices_kernel(const float* logits, long long ld, int vocab, const float* sc
         const int e0 = 4 * v - s.shift;                    // the chunk's first element
         if (v < s.v1 && !s.dead) {
             const unsigned to = mine_at + stage * STAGE;
-            if (e0 >= 0 && e0 + 4 * CHUNK + 4 <= s.e_hi) { // all of it lies in the slice
+            if (e0 >= 0 && e0 + 4 * CHUNK + (s.shift ? 4 : 0) <= s.e_hi) {             // all of it lies in the slice
                 const float* from = s.row + e0 + 4 * tid;
 #pragma unroll
                 for (int i = 0; i < NV; ++i) copy_async16(to + i * STEP, from + i * (4 * ST));
@@ -600,6 +600,7 @@ RI_API int ri_beam_select(const float* logits, long long ld, int vocab, const fl
         return (int)cudaErrorInvalidValue;
     const int rows = groups * beams, slices = slices_of(rows, vocab, sms);
     const int a_slice = (vectors_of(vocab) + slices - 1) / slices;
+    if ((long long)rows * slices * picks > (1ll << 30)) return (int)cudaErrorInvalidValue;
     SliceStat* stat = (SliceStat*)scratch;
     unsigned long long* best = (unsigned long long*)(stat + (size_t)rows * slices);
     cudaStream_t s = (cudaStream_t)stream;

@@ -2056,9 +2056,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, out_scor
 
     logits fp32 [groups * beams, vocab] (unit column stride, any row stride), scores fp32 [groups * beams].  The outputs
     [groups, picks] get, best first, the scores (fp32), the rows they continue (int32, counted over all groups) and the
-    tokens (int32).  Equal scores go by ascending (row, token); scores are compared in 64 bits.  A row whose score is -inf
-    has no continuation but of score -inf, and neither has a token whose logit is -inf or not a number.  In a row that
-    holds +inf, those tokens share the weight.  Up to 64 beams and 128 picks."""
+    tokens (int32).  Equal scores go by ascending (row, token); scores are compared in 64 bits.  A running score is finite
+    or -inf; a row whose score is -inf or not a number has no continuation but of score -inf, and neither has a token whose
+    logit is -inf or not a number.  In a row that holds +inf, those tokens share the weight.  Up to 64 beams and 128 picks."""
     _here("beam_select", logits, scores, out_scores, out_rows, out_tokens)
     if logits.dtype != torch.float32 or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise KernelError("beam_select: logits are fp32 [rows, vocab] with unit column stride")
@@ -2179,7 +2179,7 @@ def attention_decode_beams(q: torch.Tensor, out: torch.Tensor, cache: torch.Tens
 
     q, out bf16 [rows, heads * head_dim] (unit column stride), cache bf16 [pages, 2, kv heads, page, head_dim], block_table int32
     [rows, pages a row] (a row has no more keys than its pages hold), kv_len int32 [rows], shared_len int32 [rows / beams].  A row
-    without keys gets zeros.  A group one of whose rows has fewer keys than shared_len, or whose rows' windows start at different
+    without keys gets zeros; a page number outside the cache stands for a page of zeros.  A group one of whose rows has fewer keys than shared_len, or whose rows' windows start at different
     keys, is read row by row.  most_shared and most_own: about how many keys the longest shared part and the longest rest have
     (they choose how the work is cut, not what is computed).  part_o, part_lse: fp32 scratch (`decode_scratch_floats` with the
     sum of `attention_beams_splits`, at most BEAM_SPLITS_MAX); without them it is allocated."""

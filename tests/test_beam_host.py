@@ -272,3 +272,14 @@ def test_params_are_checked():
     for kw in (dict(beams=0), dict(beams=65), dict(best=0), dict(beams=2, best=3), dict(max_tokens=0), dict(length_penalty=float("nan"))):
         with pytest.raises(ValueError):
             BeamParams(**kw).validate()
+
+
+def test_the_operators_refuse_what_is_not_on_the_device():
+    import torch
+    from rustinfer_b200.ops import kernels as K
+    from rustinfer_b200.ops.library import KernelError
+    f, i = torch.zeros((4, 50)), torch.zeros(4, dtype=torch.int32)
+    for call in (lambda: K.beam_select(f, f[0, :4], 2, f[:2, :3], i, i), lambda: K.reorder_rows(f, i, i, 2), lambda: K.copy_pages(f, i, i),
+                 lambda: K.attention_decode_beams(f, f, f, f, i, i, 2, 1, 1, 16, 1.0, None, 1, 1)):
+        with pytest.raises(KernelError):
+            call()

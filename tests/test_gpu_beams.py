@@ -128,6 +128,16 @@ def test_choice_from_rows_off_their_boundaries(K, offset, ld):
     _agree(_select(K, logits, scores, 3, 9), _best(logits.cpu().numpy(), scores.cpu().numpy(), 3, 9), vocab)
 
 
+def test_choice_from_rows_that_lie_beyond_32_bits(K):
+    """Rows more than 2^31 elements apart."""
+    rows, vocab, ld = 2, 9001, (1 << 31) + 6
+    flat = torch.empty(ld + vocab, device="cuda")
+    logits = flat.as_strided((rows, vocab), (ld, 1))
+    logits.copy_(torch.randn((rows, vocab), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda"))
+    scores = torch.tensor([-1.0, -1.5], device="cuda")
+    _agree(_select(K, logits, scores, 2, 20), _best(logits.cpu().numpy(), scores.cpu().numpy(), 2, 20), vocab)
+
+
 def test_choice_refuses(K):
     x, s = torch.randn((4, 50), device="cuda"), torch.zeros(4, device="cuda")
 
@@ -394,6 +404,40 @@ def test_attention_of_beams_reads_nothing_behind_a_rows_end(K):
     assert int(kv_len[8]) == 0 and torch.all(out[8] == 0)
 
 
+@pytest.mark.parametrize("dim", [64, 48])
+def test_attention_of_beams_over_a_cache_beyond_32_bits(K, dim):
+    """Pages that start past 2^31 elements and 2^32 bytes."""
+    heads, kv_heads, beams, page, count = 8, 8, 2, 16, (1 << 31) // (2 * 8 * 16 * dim) + 60
+    q, small, table, kv_len, sh = _beams(1, beams, heads, kv_heads, dim, page, [200], [[9, 30]], seed=2)
+    cache = torch.empty((count, 2, kv_heads, page, dim), dtype=torch.bfloat16, device="cuda")
+    cache[count - small.shape[0]:] = small
+    table = torch.where(table < 0, table, table + count - small.shape[0])
+    out = torch.empty_like(q)
+    K.attention_decode_beams(q, out, cache, table.clamp(min=0), kv_len, sh, beams, heads, kv_heads, dim, 0.125, None, 200, 30)
+    _near(out, *_attention(q, cache, table, kv_len, heads, kv_heads, dim, 0.125, None), dim, 230)
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 8), (64, 5), (48, 16)])
+def test_attention_of_beams_with_pages_that_do_not_exist(K, dim, page):
+    """Numbers outside the cache, in the shared part and in a row's own: pages of zeros."""
+    heads, kv_heads, beams = 4, 2, 3
+    q, cache, table, kv_len, sh = _beams(2, beams, heads, kv_heads, dim, page, [150, 70], [[40, 33, 21], [5, 1, 30]], seed=dim)
+    zeros = int((set(range(cache.shape[0])) - set(table[table >= 0].tolist())).pop())
+    cache[zeros] = 0
+    for r, b, bad in ((0, 2, -1), (0, 3, 1 << 30), (1, 150 // page + 1, cache.shape[0]), (4, 1, -7), (5, 70 // page + 1, -(1 << 31))):
+        if r in (0, 4):                                    # shared blocks: the whole group's
+            rows = range(0, 3) if r == 0 else range(3, 6)
+            for i in rows:
+                table[i, b] = bad
+        else:
+            table[r, b] = bad
+    used = torch.arange(table.shape[1], device="cuda")[None] * page < kv_len[:, None]
+    want_table = torch.where((table < 0) | (table >= cache.shape[0]), zeros, table)
+    out = torch.empty_like(q)
+    K.attention_decode_beams(q, out, cache, torch.where(used, table, 0), kv_len, sh, beams, heads, kv_heads, dim, 0.125, None, 150, 40)
+    _near(out, *_attention(q, cache, want_table, kv_len, heads, kv_heads, dim, 0.125, None), dim, 200)
+
+
 def test_attention_of_beams_passes_on_what_is_no_number(K):
     q, cache, table, kv_len, sh = _beams(2, 2, 4, 2, 64, 16, [90, 90], [[9, 9], [9, 9]], seed=1)
     cache[int(table[0, 2]), 1, 0, 3, 5] = math.nan         # a shared value of the first group, key head 0
@@ -441,6 +485,19 @@ def test_attention_of_beams_refuses(K):
                dict(part_o=torch.empty(3, device="cuda"), part_lse=torch.empty(3, device="cuda"))):
         _refused(call(**kw))
     K.attention_decode_beams(q[:0], q[:0].clone(), cache, table[:0], kv_len[:0], sh[:0], 2, 4, 2, 64, 0.1, None, 1, 1)
+
+
+def test_tensors_of_another_device_are_refused(K, monkeypatch):
+    """As if the current device were another one than the tensors'."""
+    from rustinfer_b200.ops import library
+    q, cache, table, kv_len, sh = _beams(1, 2, 4, 2, 64, 16, [20], [[3, 3]])
+    i32 = torch.zeros(2, dtype=torch.int32, device="cuda")
+    x = torch.randn((2, 40), device="cuda")
+    monkeypatch.setattr(library, "_current_device", lambda: 1)
+    _refused(lambda: K.beam_select(x, x[:, 0].contiguous(), 2, x[:1, :2].contiguous(), i32[None], i32[None]))
+    _refused(lambda: K.reorder_rows(x[None], i32, i32, 2))
+    _refused(lambda: K.copy_pages(x[None], i32, i32))
+    _refused(lambda: K.attention_decode_beams(q, q.clone(), cache, table.clamp(min=0), kv_len, sh, 2, 4, 2, 64, 0.1, None, 20, 3))
 
 
 # ------------------------------------------------------------------------------------- together, and elsewhere than on the default stream
