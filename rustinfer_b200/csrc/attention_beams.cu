@@ -170,7 +170,6 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
     bf16* Qs = KVs + STAGES * STAGE;                       // [RTILES * 16][ROW]
     uint64_t* full = reinterpret_cast<uint64_t*>(Qs + RTILES * 16 * ROW);
     const int rt = warp / KG, kg = warp % KG;
-    const bool works = warp < RTILES * KG;
     // where a lane's fragments lie in a stage, in bytes: a row of keys and one of values.  By TMA, columns 16 ks on are an exclusive or away
     // (the swizzle's bits are the only ones below a row), 64 columns a block; else 32 bytes a step
     const int k_row = kg * WK + (lane & 7) + (lane >> 4) * 8, v_row = kg * WK + (lane & 15);
@@ -244,6 +243,13 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
             if (t + 1 < tiles) look_up(t + 1);
         }
     };
+    // queries, all on their way at once (loaded and stored one after the other they were half of the time to the first tile); the first
+    // tile's group takes them in, by TMA they are their own
+    for (int c = tid; c < RTILES * 16 * CH; c += THREADS) {
+        const int r = c / CH, ch = c - r * CH, m = m0 + min(r, m_count - 1), b = m / G;
+        cp_async16(Qs + r * ROW + ch * 8, a.q + (size_t)(g * a.beams + b) * a.q_stride + (size_t)(kvh * G + m - b * G) * HD + ch * 8, r < m_count);
+    }
+    if constexpr (TMA) cp_async_commit();
     if constexpr (TMA) {
         if (tid == 0) {
             for (int s = 0; s < STAGES; ++s) bar_init(&full[s]);
@@ -261,19 +267,11 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
         if (s < tiles) fetch(s, s);
         if constexpr (!TMA) cp_async_commit();
     }
-    for (int c = tid; c < RTILES * 16 * CH; c += THREADS) {
-        const int r = c / CH, ch = c - r * CH, m = m0 + r;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (r < m_count) {
-            const int b = m / G, h = m - b * G;
-            v = *reinterpret_cast<const uint4*>(a.q + (size_t)(g * a.beams + b) * a.q_stride + (size_t)(kvh * G + h) * HD + ch * 8);
-        }
-        *reinterpret_cast<uint4*>(Qs + r * ROW + ch * 8) = v;
-    }
     float o[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    if constexpr (TMA) cp_async_wait<0>();
     __syncthreads();                                       // queries are there, and the barriers
 
     unsigned parity = 0;
@@ -299,7 +297,7 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
         const unsigned stage_at = base + stage * (STAGE * 2);
         if (++stage == STAGES) { stage = 0; parity ^= 1u; }
         const int kw0 = kg * WK, key0 = (t0 + t) * KT + kw0;
-        if (!works || key0 >= hi || key0 + WK <= lo) continue;
+        if (key0 >= hi || key0 + WK <= lo) continue;
         const bool edge = key0 < lo || key0 + WK > hi;
         if constexpr (TMA) {
             if (edge) {
@@ -387,50 +385,68 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
         }
     }
     if constexpr (!TMA) cp_async_wait<0>();
-    __syncthreads();
 
-    // the warps' states through shared memory (the tiles are used up)
-    float* Os = reinterpret_cast<float*>(KVs);             // [WARPS][16][OROW]
-    float* Ms = Os + WARPS * 16 * OROW;                    // [WARPS][16]
-    float* Ls = Ms + WARPS * 16;
-    if (works)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    }
+    auto part_of = [&](int r) -> size_t {                  // of row m0 + r
+        const int mm = m0 + r, b = mm / G;
+        return ((size_t)(g * a.beams + b) * a.Hq + kvh * G + mm - b * G) * splits + part;
+    };
+    if constexpr (KG == 1) {                               // a row's keys are one warp's: from its registers
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+            const int r = rt * 16 + (lane >> 2) + 8 * i;
+            if (r < m_count) {
+                const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+                const size_t p = part_of(r);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    *reinterpret_cast<float2*>(a.part_o + p * HD + n * 8 + (lane & 3) * 2) = make_float2(o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
+                if ((lane & 3) == 0) a.part_lse[p] = l[i] == 0.f ? -INFINITY : (m[i] == -INFINITY ? 0.f : m[i]) + log2f(l[i]);
+            }
+        }
+    } else {
+        // the warps' states through shared memory (the tiles are used up)
+        __syncthreads();
+        float* Os = reinterpret_cast<float*>(KVs);         // [WARPS][16][OROW]
+        float* Ms = Os + WARPS * 16 * OROW;                // [WARPS][16]
+        float* Ls = Ms + WARPS * 16;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
             const int r = (lane >> 2) + 8 * i;
             float* orow = Os + (warp * 16 + r) * OROW + (lane & 3) * 2;
 #pragma unroll
             for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(orow + n * 8) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
             if ((lane & 3) == 0) { Ms[warp * 16 + r] = m[i]; Ls[warp * 16 + r] = l[i]; }
         }
-    __syncthreads();
-    for (int r = warp; r < m_count; r += WARPS) {          // a warp a row
-        const int w0 = (r >> 4) * KG, rr = r & 15;
-        float M = -INFINITY;
+        __syncthreads();
+        constexpr int FOURS = RTILES * 16 * (HD / 4);      // four outputs a thread at a time
 #pragma unroll
-        for (int w = 0; w < KG; ++w) M = fmaxf(M, Ms[(w0 + w) * 16 + rr]);
-        const float muse = M == -INFINITY ? 0.f : M;
-        float f[KG], L = 0.f;
+        for (int c0 = 0; c0 < FOURS; c0 += THREADS) {
+            const int c = c0 + tid, r = c / (HD / 4), d = (c - r * (HD / 4)) * 4;
+            if (c >= FOURS || r >= m_count) continue;
+            const int w0 = (r >> 4) * KG, rr = r & 15;
+            float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < KG; ++w) {
-            const float lw = Ls[(w0 + w) * 16 + rr];
-            f[w] = lw == 0.f ? 0.f : ex2(Ms[(w0 + w) * 16 + rr] - muse);
-            L += lw * f[w];
-        }
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        const int mm = m0 + r, b = mm / G, h = mm - b * G;
-        const size_t p = ((size_t)(g * a.beams + b) * a.Hq + kvh * G + h) * splits + part;
-        for (int d = lane * 4; d < HD; d += 128) {
+            for (int w = 0; w < KG; ++w) M = fmaxf(M, Ms[(w0 + w) * 16 + rr]);
+            const float muse = M == -INFINITY ? 0.f : M;
+            float L = 0.f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < KG; ++w) {
+                const float lw = Ls[(w0 + w) * 16 + rr], f = lw == 0.f ? 0.f : ex2(Ms[(w0 + w) * 16 + rr] - muse);
+                L += lw * f;
                 const float4 x = *reinterpret_cast<const float4*>(Os + ((w0 + w) * 16 + rr) * OROW + d);
-                if (f[w] != 0.f) { v.x += x.x * f[w]; v.y += x.y * f[w]; v.z += x.z * f[w]; v.w += x.w * f[w]; }
+                if (f != 0.f) { v.x += x.x * f; v.y += x.y * f; v.z += x.z * f; v.w += x.w * f; }
             }
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            const size_t p = part_of(r);
             *reinterpret_cast<float4*>(a.part_o + p * HD + d) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+            if (d == 0) a.part_lse[p] = L == 0.f ? -INFINITY : muse + log2f(L);                   // what is no number stays none
         }
-        if (lane == 0) a.part_lse[p] = L == 0.f ? -INFINITY : muse + log2f(L);               // what is no number stays none
     }
 }
 
@@ -672,24 +688,29 @@ beams_join_kernel(const float* part_o, const float* part_lse, bf16* out, int out
     float4 v[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int AT_ONCE = V == 1 ? 8 : 4;                // ranges whose loads are in flight together
     for (unsigned some = __ballot_sync(0xffffffffu, lse != -INFINITY); some;) {
-        // two ranges' loads in flight together
-        const int s0 = __ffs(some) - 1;
-        some &= some - 1;
-        const int s1 = some ? __ffs(some) - 1 : -1;
-        some &= some - 1;
-        const float w0 = __shfl_sync(0xffffffffu, w, s0), w1 = __shfl_sync(0xffffffffu, w, max(0, s1));
+        float4 x[AT_ONCE][V];
+        float ws[AT_ONCE];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int d = lane * 4 + i * 128;
-            if (d < HD) {
-                const float4 x = *reinterpret_cast<const float4*>(part_o + (p + s0) * HD + d);
-                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (s1 >= 0) y = *reinterpret_cast<const float4*>(part_o + (p + s1) * HD + d);
-                v[i].x += w0 * x.x; v[i].y += w0 * x.y; v[i].z += w0 * x.z; v[i].w += w0 * x.w;
-                if (s1 >= 0) { v[i].x += w1 * y.x; v[i].y += w1 * y.y; v[i].z += w1 * y.z; v[i].w += w1 * y.w; }
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const int s = __ffs(some) - 1;                 // -1: none is left
+            some &= some - 1;
+            ws[k] = __shfl_sync(0xffffffffu, w, max(0, s));
+            if (s < 0) ws[k] = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int d = lane * 4 + i * 128;
+                x[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (s >= 0 && d < HD) x[k][i] = *reinterpret_cast<const float4*>(part_o + (p + s) * HD + d);
             }
         }
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                v[i].x += ws[k] * x[k][i].x; v[i].y += ws[k] * x[k][i].y; v[i].z += ws[k] * x[k][i].z; v[i].w += ws[k] * x[k][i].w;
+            }
     }
     const int r = id / Hq, h = id - r * Hq;
     bf16* to = out + (size_t)r * out_stride + (size_t)h * HD;
