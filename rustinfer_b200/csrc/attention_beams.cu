@@ -37,6 +37,7 @@ constexpr int THREADS = 32 * WARPS;
 constexpr int CTAS = HD <= 64 ? 4 : HD <= 128 ? 2 : 1;     // CTAs an SM that registers and shared memory are cut for
 constexpr int MAX_BEAMS = 64;
 constexpr int OWN_KEYS = 16;                               // keys of its own a row's warp takes at a time
+constexpr int OWN_STAGES = 2;                              // of which so many are on their way
 constexpr bool BY_TMA = HD == 64 || HD == 128;
 constexpr int TKB_OR_1 = BY_TMA ? HD / 64 : 1;             // 64-column blocks of a head
 constexpr int NO_KEY = (int)0x80000000;                    // in place of a page
@@ -455,7 +456,8 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
 __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, int r, int kvh, int head0, int heads, int lo, int hi, int part) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int splits = a.shared_splits + a.own_splits;
-    bf16* Ks = reinterpret_cast<bf16*>(smem) + warp * 2 * OWN_KEYS * ROW;
+    constexpr int BUFFER = 2 * OWN_KEYS * ROW;             // elements: keys, then values
+    bf16* Ks = reinterpret_cast<bf16*>(smem) + warp * OWN_STAGES * BUFFER;
     bf16* Vs = Ks + OWN_KEYS * ROW;
     const unsigned k_at = smem_u32(Ks) + (((lane & 7) + (lane >> 4) * 8) * ROW + ((lane >> 3) & 1) * 8) * 2;
     const unsigned v_at = smem_u32(Vs) + ((lane & 15) * ROW + (lane >> 4) * 8) * 2;
@@ -482,9 +484,12 @@ __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, i
         if (lane < heads) a.part_lse[p0 + (size_t)lane * splits] = -INFINITY;
         return;
     }
-    int page = look_up(lo), page_then = look_up(lo + OWN_KEYS);
+    int page = look_up(lo), page_then = look_up(lo + OWN_KEYS), page_later = look_up(lo + 2 * OWN_KEYS);
     fetch(Ks, lo, page, 0);
     fetch(Vs, lo, page, value_step);
+    fetch(Ks + BUFFER, lo + OWN_KEYS, page_then, 0);       // (keys from hi on: zeros, nothing is read)
+    fetch(Vs + BUFFER, lo + OWN_KEYS, page_then, value_step);
+    page = page_later;
     unsigned qf[KS][2];                                    // rows 0 to 7 alone
     {
         const int h = lane >> 2;
@@ -499,21 +504,20 @@ __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, i
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = 0.f;
     float m = -INFINITY, l = 0.f;
-    for (int k0 = lo; k0 < hi; k0 += OWN_KEYS) {
-        cp_async_wait<1>();
+    for (int k0 = lo, buffer = 0; k0 < hi; k0 += OWN_KEYS, buffer ^= BUFFER) {
+        cp_async_wait<2 * OWN_STAGES - 1>();
         __syncwarp();
         float s[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             unsigned kf[4];
-            ldmatrix_x4(kf, k_at + ks * 32);
+            ldmatrix_x4(kf, k_at + buffer * 2 + ks * 32);
             mma_8rows(s[0], qf[ks][0], qf[ks][1], kf[0], kf[1]);
             mma_8rows(s[1], qf[ks][0], qf[ks][1], kf[2], kf[3]);
         }
         __syncwarp();
-        page = page_then;
-        page_then = look_up(k0 + 2 * OWN_KEYS);
-        if (k0 + OWN_KEYS < hi) fetch(Ks, k0 + OWN_KEYS, page, 0);
+        page_later = look_up(k0 + (OWN_STAGES + 1) * OWN_KEYS);
+        if (k0 + OWN_STAGES * OWN_KEYS < hi) fetch(Ks + buffer, k0 + OWN_STAGES * OWN_KEYS, page, 0);
         else cp_async_commit();
         float mx = -INFINITY;
 #pragma unroll
@@ -540,20 +544,21 @@ __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, i
         unsigned ph[2], pl[2];
         two_pieces(s[0][0], s[0][1], ph[0], pl[0]);
         two_pieces(s[1][0], s[1][1], ph[1], pl[1]);
-        cp_async_wait<1>();
+        cp_async_wait<2 * OWN_STAGES - 1>();
         __syncwarp();
 #pragma unroll
         for (int np = 0; np < NT / 2; ++np) {
             unsigned vf[4];
-            ldmatrix_x4_trans(vf, v_at + np * 32);
+            ldmatrix_x4_trans(vf, v_at + buffer * 2 + np * 32);
             mma_8rows(o[2 * np], ph[0], ph[1], vf[0], vf[1]);
             mma_8rows(o[2 * np + 1], ph[0], ph[1], vf[2], vf[3]);
             mma_8rows(o[2 * np], pl[0], pl[1], vf[0], vf[1]);
             mma_8rows(o[2 * np + 1], pl[0], pl[1], vf[2], vf[3]);
         }
         __syncwarp();
-        if (k0 + OWN_KEYS < hi) fetch(Vs, k0 + OWN_KEYS, page, value_step);
+        if (k0 + OWN_STAGES * OWN_KEYS < hi) fetch(Vs + buffer, k0 + OWN_STAGES * OWN_KEYS, page, value_step);
         else cp_async_commit();
+        page = page_later;
     }
     cp_async_wait<0>();
     l += __shfl_xor_sync(0xffffffffu, l, 1);
@@ -729,7 +734,7 @@ beams_join_kernel(const float* part_o, const float* part_lse, bf16* out, int out
 template <int RTILES, bool TMA>
 constexpr size_t smem_bytes() {
     const size_t kv = (size_t)STAGES * 2 * KT * (TMA ? HD : ROW) * sizeof(bf16) + (size_t)RTILES * 16 * ROW * sizeof(bf16) + 64;
-    const size_t merge = (WARPS * 16 * (size_t)OROW + 2 * WARPS * 16) * sizeof(float), own = (size_t)WARPS * 2 * OWN_KEYS * ROW * sizeof(bf16);
+    const size_t merge = (WARPS * 16 * (size_t)OROW + 2 * WARPS * 16) * sizeof(float), own = (size_t)WARPS * OWN_STAGES * 2 * OWN_KEYS * ROW * sizeof(bf16);
     return 1024 /*alignment*/ + (kv > merge ? (kv > own ? kv : own) : (merge > own ? merge : own));
 }
 
