@@ -267,8 +267,8 @@ class ModelRunner:
     """Model, cache and step function of one model folder on one GPU."""
 
     # Steps of beams read their requests' common keys once when all beams together see at least so many of them: below, the rows' own
-    # kernel, whose later rows find them in L2, is sooner (us a layer of 8 key heads of 64, rows / beams: 64 rows behind 300 keys 9 / 14,
-    # behind 1,000 19 / 18, behind 4,000 61 / 28; 8 rows behind 4,000 14 / 18)
+    # kernel, whose later rows find them in L2, is sooner (us a layer of 8 key heads of 64, rows / beams: 64 rows behind 300 keys 9 / 13,
+    # behind 1,000 18 / 17, behind 4,000 61 / 26; 8 rows behind 4,000 14 / 15)
     beam_keys = 64 * 1024
 
     def __init__(self, model_dir: str, dtype="bfloat16", device="cuda:0", max_model_len: int = 4096,

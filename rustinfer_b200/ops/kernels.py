@@ -2150,23 +2150,33 @@ BEAM_SPLITS_MAX = 20          # ranges of a row's keys at most: 16 of shared one
 
 def attention_beams_splits(most_shared: int, most_own: int) -> Tuple[int, int]:
     """Ranges there is room for of a group's shared keys, and ranges a row's own keys are cut into, for about so many keys."""
-    return max(1, min(-(-most_shared // 64), 16)), max(1, min(-(-most_own // 32), 4))
+    return max(1, min(-(-most_shared // 64), 16)), max(1, min(most_own // 96, 4))
 
 
 @functools.lru_cache(maxsize=4096)
 def _attention_beams_plan(rows: int, beams: int, num_heads: int, num_kv_heads: int, head_dim: int, most_shared: int, most_own: int, num_sms: int):
     """(entry point, ranges of shared keys, of own ones, CTAs for the former, floats of partial results and of their log-sum-exps).  The CTAs
-    that read shared keys are those that run at once, less a quarter of the ones that read the rows' own (4 x 16 beams of 9,001 and 300
-    keys: without the latter 71 us, less them all 84; 8 x 8 of 4,096 and 60: 35 and 42)."""
+    that read shared keys start first and are the most eighths of those that run at once, 7 at most and 2 at least, whose time leaves the rest
+    enough of it for the rows' own keys: by about 6 us and 2 a tile of 64 keys for the former, 3 us and 1 a step of 16 for a row's warp, both
+    for heads of 64.  (Over 23 shapes 3 % behind the best cut of each, 9 % at most.  us, against a fixed 6 or 7 eighths with ranges of 32 own
+    keys: 4 x 16 beams, heads of 128, of 9,001 and 100 keys 44 and 53, of 2,000 and 300 31 and 36, of 9,001 and 1,000 71 and 84; 8 x 8,
+    heads of 64, of 4,096 and 1,000 52 and 62.)"""
     if not attention_beams_supports(num_heads, num_kv_heads, head_dim):
         raise KernelError(f"attention_decode_beams: {num_heads} heads over {num_kv_heads} of {head_dim} (a multiple of 16 up to {L.MMA_MAX_HEAD_DIM})")
     if not 1 <= beams <= BEAMS_MAX or rows % beams:
         raise KernelError(f"attention_decode_beams: {rows} rows are no groups of {beams} (1 to {BEAMS_MAX})")
     lib = L.attention_beams(head_dim)
     shared, own = attention_beams_splits(most_shared, most_own)
-    at_once = int(lib.ri_attention_beams_ctas_per_sm()) * num_sms
-    own_ctas = -(-rows * num_kv_heads * -(-(num_heads // num_kv_heads) // 8) * own // 4)
-    return (lib.ri_attention_beams, shared, own, at_once - min(at_once // 4, own_ctas // 4), *decode_scratch_floats(rows, num_heads, head_dim, shared + own))
+    at_once, size, group = int(lib.ri_attention_beams_ctas_per_sm()) * num_sms, head_dim / 64, num_heads // num_kv_heads
+    chunks = -(-beams * group // (16 * int(lib.ri_attention_beams_row_tiles(beams * group))))
+    tiles = rows // beams * -(-max(1, most_shared) // 64) * num_kv_heads * chunks
+    own_ctas = -(-rows * num_kv_heads * -(-group // 8) * own // 4)
+    own_time = own_ctas * (3 + -(-most_own // (16 * own)) * size)
+    for eighths in range(7, 1, -1):
+        ctas = max(1, at_once * eighths // 8)
+        if (at_once - ctas) * (6 + 2 * size * tiles / ctas) >= own_time:
+            break
+    return (lib.ri_attention_beams, shared, own, ctas, *decode_scratch_floats(rows, num_heads, head_dim, shared + own))
 
 
 def attention_decode_beams(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,
@@ -2185,8 +2195,8 @@ def attention_decode_beams(q: torch.Tensor, out: torch.Tensor, cache: torch.Tens
     sum of `attention_beams_splits`, at most BEAM_SPLITS_MAX); without them it is allocated."""
     _here("attention_decode_beams", q, out, cache, block_table, kv_len, shared_len, part_o, part_lse)
     R, width = q.shape[0], num_heads * head_dim
-    entry, shared, own, ctas, need_o, need_l = _attention_beams_plan(R, beams, num_heads, num_kv_heads, head_dim, max(0, int(most_shared)),
-                                                                     max(1, int(most_own)), L.num_sms(q.device))
+    entry, shared, own, ctas, need_o, need_l = _attention_beams_plan(R, beams, num_heads, num_kv_heads, head_dim, max(0, int(most_shared if window is None else min(most_shared, window + 64))), max(1, int(most_own)),
+                                                                     L.num_sms(q.device))
     bf16, i32 = torch.bfloat16, torch.int32
     q_step, out_step = q.stride(0), out.stride(0)
     if (q.dtype != bf16 or out.dtype != bf16 or q.shape != (R, width) or out.shape != (R, width) or q.stride(1) != 1 or out.stride(1) != 1
