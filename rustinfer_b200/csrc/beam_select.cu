@@ -32,8 +32,8 @@ constexpr int STAGES = 2;                                  // chunks of a slice 
 // half the size 81.  The logits' stream with its sums alone takes 48)
 constexpr int MAX_CHUNKS = 8;                              // chunks of a slice
 constexpr int LISTS = 1024;                                // slices of a group whose sums are kept in shared memory
-constexpr int KEPT = 16384;                                // ... and elements of the pool whose rounded scores are
 constexpr int MT = 512;                                    // threads of a group
+constexpr int PLACES = 8192;                               // of a group's pool that shared memory holds
 constexpr int CAP = 1024;                                  // room of the gathering
 constexpr int MAX_PICKS = 128, MAX_BEAMS = 64;
 
@@ -99,6 +99,10 @@ __device__ __forceinline__ void copy_async16(unsigned to, const void* from) {
 }
 __device__ __forceinline__ void copy_async4(unsigned to, const void* from) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_async8(unsigned to, const void* from, bool there) {       // else zeros
+    const int n = there ? 8 : 0;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(to), "l"(from), "r"(n) : "memory");
 }
 
 __global__ void __launch_bounds__(ST, CTAS)
@@ -392,11 +396,11 @@ __global__ void __launch_bounds__(MT)
 beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const float* scores,
                   int vocab, int beams, int slices, int picks, float* out_scores, int* out_rows,
                   int* out_tokens) {
-    extern __shared__ unsigned rounded[];                  // [lists][room], where they fit
+    extern __shared__ unsigned long long pool[];           // [lists][room, as a power of two], where they fit; 0: no element.  Their rounded scores behind
     __shared__ double base[MAX_BEAMS], so_far[MAX_BEAMS];  // log of the row's sum; its score
     __shared__ float row_top[MAX_BEAMS];
     __shared__ double l_score[CAP];
-    __shared__ long long l_flat[CAP];
+    __shared__ long long l_at[CAP];                        // row of the group << 32 | token
     __shared__ SliceStat held[LISTS];
     __shared__ unsigned wmax[MT / 32], wmin[MT / 32];
     __shared__ unsigned long long best_of[MT / 32];
@@ -410,7 +414,22 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
     for (int l = tid; l < min(lists, LISTS); l += MT) held[l] = of[l];
     __syncthreads();
     auto stat_of = [&](int l) -> SliceStat { return l < LISTS ? held[l] : of[l]; };
+    // A pool that fits is read once, all of it on its way while the sums are made; its lists lie 1 << places apart.  (1 x 4 beams of 128,256 words
+    // 12.4 -> 8.8 us, 32 x 16 with 48 picks 69 -> 66.5: loads that wait for the sums, and a second read of what is taken)
+    const int places = 32 - __clz(room - 1);
+    const bool fits = lists <= PLACES >> places;
+    const int all = fits ? lists << places : 0;
+    if (fits) {
+        const unsigned to = (unsigned)__cvta_generic_to_shared(pool);
+#pragma unroll 4
+        for (int at = tid; at < all; at += MT) {
+            const int l = at >> places, k = at & ((1 << places) - 1);
+            const bool there = k < stat_of(l).n;
+            copy_async8(to + 8 * at, there ? keys + (size_t)l * room + k : keys, there);
+        }
+    }
     for (int b = warp; b < beams; b += MT / 32) {
+        const float before = scores[(size_t)g * beams + b];
         float m = -INFINITY;
         for (int i = lane; i < slices; i += 32) m = fmaxf(m, stat_of(b * slices + i).m);
         m = warp_max(m);
@@ -435,14 +454,14 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
             // log of the row's sum; that L is not log2 e to the last bit acts as a factor of the logits, here of the largest
             const double l = log(sum);
             row_top[b] = m;
-            so_far[b] = (double)scores[(size_t)g * beams + b];
+            so_far[b] = (double)before;
             base[b] = m == INFINITY      ? l
                       : by_difference(m) ? (double)m + l
                                          : l + 0.6931471805599453 * ref + (double)m * (1.0 - 0.6931471805599453 * (double)L);
         }
     }
     __syncthreads();
-    // every element of the pool once: a warp four lists, whose loads are in flight together
+    // every element of a pool that does not fit, or more than once: a warp four lists, whose loads are in flight together
     auto each = [&](auto use) {
         constexpr int AT_ONCE = 4;
         for (int l0 = warp; l0 < lists; l0 += AT_ONCE * (MT / 32)) {
@@ -459,7 +478,7 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
                 for (int q = 0; q < AT_ONCE; ++q) key[q] = k < n[q] ? keys[(size_t)(l0 + q * (MT / 32)) * room + k] : 0ull;
 #pragma unroll
                 for (int q = 0; q < AT_ONCE; ++q)
-                    if (key[q]) use((l0 + q * (MT / 32)) / slices, key[q], (l0 + q * (MT / 32)) * room + k);
+                    if (key[q]) use((l0 + q * (MT / 32)) / slices, key[q]);
             }
         }
     };
@@ -473,14 +492,24 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
     auto flat_of = [&](int b, unsigned long long key) -> long long {
         return (long long)b * vocab + (long long)(0xffffffffu - (unsigned)(key & 0xffffffffu));
     };
+    asm volatile("cp.async.wait_all;\n" ::: "memory");     // (a thread reads what it has fetched itself)
     // 32-bit keys for the search: rounding keeps the order, and equals after rounding are all gathered
     unsigned mine = 0;
-    const bool kept = lists * room <= KEPT;
-    each([&](int b, unsigned long long key, int at) {
-        const unsigned o = ordered((float)score_of(b, key));
-        if (kept) rounded[at] = o;
-        mine = max(mine, o);
-    });
+    // (l + 1/2) / slices rounds down to l's row: l is below 2^13, so it is off by 2^-9 of 1 / slices at most, and half of that away from a whole number
+    const float a_row = 1.f / (float)slices;
+    auto row_of = [&](int at) -> int { return (int)(((float)(at >> places) + 0.5f) * a_row); };
+    unsigned* const rounded = reinterpret_cast<unsigned*>(pool + all);
+    if (fits) {
+#pragma unroll 4
+        for (int at = tid; at < all; at += MT) {
+            const unsigned long long key = pool[at];
+            const unsigned o = key ? ordered((float)score_of(row_of(at), key)) : 0u;
+            rounded[at] = o;
+            mine = max(mine, o);
+        }
+    } else {
+        each([&](int b, unsigned long long key) { mine = max(mine, ordered((float)score_of(b, key))); });
+    }
     unsigned top = __reduce_max_sync(0xffffffffu, mine);
     const unsigned low = __reduce_min_sync(0xffffffffu, mine ? mine : 0xffffffffu);
     if (lane == 0) { wmax[warp] = top; wmin[warp] = low; }
@@ -490,16 +519,14 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
     if (lists > 1) t = reach(mine, t, top, picks);
     auto take = [&](int b, unsigned long long key) {
         const int at = atomicAdd(&listed, 1);
-        if (at < CAP) { l_score[at] = score_of(b, key); l_flat[at] = flat_of(b, key); }
+        if (at < CAP) { l_score[at] = score_of(b, key); l_at[at] = (long long)b << 32 | (0xffffffffu - (unsigned)(key & 0xffffffffu)); }
     };
-    if (kept) {                                            // what reaches t is read again, the rest is not
-        for (int l = warp; l < lists; l += MT / 32) {
-            const int n = stat_of(l).n;
-            for (int k = lane; k < n; k += 32)
-                if (rounded[l * room + k] >= t) take(l / slices, keys[(size_t)l * room + k]);
-        }
+    if (fits) {
+#pragma unroll 4
+        for (int at = tid; at < all; at += MT)
+            if (rounded[at] >= t) take(row_of(at), pool[at]);                                  // (t is 1 at least)
     } else {
-        each([&](int b, unsigned long long key, int) {
+        each([&](int b, unsigned long long key) {
             if (ordered((float)score_of(b, key)) >= t) take(b, key);
         });
     }
@@ -513,7 +540,7 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
         };
         auto count_of = [&](auto belongs) -> int {
             int c = 0;
-            each([&](int b, unsigned long long key, int) { c += belongs(ordered64(score_of(b, key) + 0.0), flat_of(b, key)); });
+            each([&](int b, unsigned long long key) { c += belongs(ordered64(score_of(b, key) + 0.0), flat_of(b, key)); });
             return block_count(c, &cell);
         };
         // asked first: whether it is -inf (most words forbidden), or all are equals of the best (the next of two probes)
@@ -525,7 +552,7 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
             probe = lo + (hi - lo) / 2 + 1;
             if (best_next && lo < hi) {
                 unsigned long long most = 0;
-                each([&](int b, unsigned long long key, int) { most = max(most, ordered64(score_of(b, key) + 0.0)); });
+                each([&](int b, unsigned long long key) { most = max(most, ordered64(score_of(b, key) + 0.0)); });
                 const unsigned high = __reduce_max_sync(0xffffffffu, (unsigned)(most >> 32));
                 const unsigned low = __reduce_max_sync(0xffffffffu, (unsigned)(most >> 32) == high ? (unsigned)most : 0u);
                 __syncthreads();
@@ -546,29 +573,26 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
         __syncthreads();
         if (tid == 0) listed = 0;
         __syncthreads();
-        each([&](int b, unsigned long long key, int) {
+        each([&](int b, unsigned long long key) {
             const double s = score_of(b, key);
             const unsigned long long o = ordered64(s + 0.0);
             const long long f = flat_of(b, key);
-            if (o > lo || (o == lo && f < f_lo)) {
-                const int at = atomicAdd(&listed, 1);
-                if (at < CAP) { l_score[at] = s; l_flat[at] = f; }
-            }
+            if (o > lo || (o == lo && f < f_lo)) take(b, key);
         });
         __syncthreads();
         n = min(listed, CAP);
     }
     for (int i = warp; i < n; i += MT / 32) {
         const double s = l_score[i];
-        const long long f = l_flat[i];
+        const long long f = l_at[i];
         int rank = 0;
-        for (int j = lane; j < n; j += 32) rank += l_score[j] > s || (l_score[j] == s && l_flat[j] < f);
+        for (int j = lane; j < n; j += 32) rank += l_score[j] > s || (l_score[j] == s && l_at[j] < f);
         rank = __reduce_add_sync(0xffffffffu, rank);
         if (lane == 0 && rank < picks) {
             const size_t at = (size_t)g * picks + rank;
             out_scores[at] = (float)s;
-            out_rows[at] = g * beams + (int)(f / vocab);
-            out_tokens[at] = (int)(f % vocab);
+            out_rows[at] = g * beams + (int)(f >> 32);
+            out_tokens[at] = (int)(f & 0xffffffff);
         }
     }
 }
@@ -610,13 +634,13 @@ RI_API int ri_beam_select(const float* logits, long long ld, int vocab, const fl
     RI_CHECKED((int)cudaGetDevice(&device));
     if (device > 63 || !(configured >> device & 1)) {
         RI_CHECKED((int)cudaFuncSetAttribute(beam_slices_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring));
-        RI_CHECKED((int)cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, KEPT * 4));
+        RI_CHECKED((int)cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PLACES * 12));
         if (device <= 63) configured |= 1ull << device;
     }
     RI_CHECKED(ri_launch(beam_slices_kernel, dim3(min(rows * slices, CTAS * sms)), dim3(ST), ring, s, logits, ld, vocab, scores, picks, rows * slices,
                          slices, a_slice, best, stat));
-    const int rounded = beams * slices * 2 * picks <= KEPT ? beams * slices * 2 * picks * 4 : 0;
-    RI_CHECKED(ri_launch(beam_merge_kernel, dim3(groups), dim3(MT), rounded, s, best, stat, scores, vocab, beams, slices, picks, out_scores, out_rows,
+    const int lists = beams * slices, places = 32 - __builtin_clz(2 * picks - 1), pool = lists <= PLACES >> places ? (lists << places) * 12 : 0;
+    RI_CHECKED(ri_launch(beam_merge_kernel, dim3(groups), dim3(MT), pool, s, best, stat, scores, vocab, beams, slices, picks, out_scores, out_rows,
                          out_tokens));
     return ri_launch_status();
 }
