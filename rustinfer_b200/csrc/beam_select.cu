@@ -28,9 +28,10 @@ constexpr int ST = 256;                                    // threads of a slice
 constexpr int NV = 4;                                      // 16-byte loads of a thread a chunk
 constexpr int CTAS = 4;                                    // CTAs an SM, which walk over slices
 constexpr int STAGES = 2;                                  // chunks of a slice in shared memory
-// (512 rows of 128,256 logits, 48 picks of 16 beams, us a call: 4 CTAs and 2 stages 69, 3 and 3 73, 3 and 2 70; 512 threads, 2 and 2 73; chunks of
+// (512 rows of 128,256 logits, 48 picks of 16 beams, slices of 8 chunks, us a call: 4 CTAs and 2 stages 69, 3 and 3 73, 3 and 2 70; 512 threads, 2 and 2 73; chunks of
 // half the size 81.  The logits' stream with its sums alone takes 48)
-constexpr int MAX_CHUNKS = 8;                              // chunks of a slice
+constexpr int MAX_CHUNKS = 16;                             // chunks of a slice
+constexpr int AGAIN = 2048;                                // threads' chunks that may be read once more
 constexpr int LISTS = 1024;                                // slices of a group whose sums are kept in shared memory
 constexpr int MT = 512;                                    // threads of a group
 constexpr int PLACES = 8192;                               // of a group's pool that shared memory holds
@@ -111,9 +112,9 @@ beam_slices_kernel(const float* logits, long long ld, int vocab, const float* sc
     extern __shared__ float4 ring[];                       // [STAGES][NV][W][33]: a warp reads what it has fetched itself, so no barrier
     __shared__ unsigned long long list[CAP];
     __shared__ unsigned red_hi[ST / 32], red_lo[ST / 32];
-    __shared__ float wsum[ST / 32];
-    __shared__ float chunk_top[MAX_CHUNKS][ST];
-    __shared__ unsigned short again[MAX_CHUNKS * ST];
+    __shared__ double wsum[ST / 32];
+    __shared__ bf16 tops[MAX_CHUNKS][ST];                       // rounded up
+    __shared__ unsigned short again[AGAIN];
     __shared__ int cell, listed;
     constexpr int W = ST / 32, CHUNK = NV * ST;
     constexpr unsigned MINUS_INF = 0x007fffffu;            // ordered(-inf)
@@ -198,15 +199,17 @@ beam_slices_kernel(const float* logits, long long ld, int vocab, const float* sc
         continue;
     }
     // A thread's sum of 2^(x L - ref), L = log2 e in 32 bits, ref a whole number that is at least the thread's largest x L: one fused
-    // multiply-add an element, whose own rounding is all that is lost, and moving on to another ref is exact.
-    float sum = 0.f, ref = -1e30f, top = -INFINITY;        // (top: what is no number does not count)
+    // multiply-add an element, whose own rounding is all that is lost, and moving on to another ref is exact.  A chunk's sixteen are
+    // added up in 32 bits, the rest in 64.
+    double sum = 0.0;
+    float ref = -1e30f, top = -INFINITY;                   // (top: what is no number does not count)
     auto add_up = [&](const float (&x)[4 * NV], float high) {
         const float to = fmaxf(ref, ceilf(high * L));
-        float part[4] = {sum * ex2(ref - to), 0.f, 0.f, 0.f};
-        ref = to;
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 4 * NV; ++i) part[i & 3] += ex2(fmaf(x[i], L, -to));
-        sum = (part[0] + part[1]) + (part[2] + part[3]);
+        sum = sum * (double)ex2(ref - to) + (double)((part[0] + part[1]) + (part[2] + part[3]));
+        ref = to;
     };
     auto highest = [&](const float (&x)[4 * NV]) {
         float h[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -259,7 +262,7 @@ beam_slices_kernel(const float* logits, long long ld, int vocab, const float* sc
         __syncwarp();                                      // the stage is free
         const float high = highest(x);
         top = fmaxf(top, high);
-        chunk_top[chunk][tid] = high;
+        tops[chunk][tid] = __float2bfloat16_ru(high);
         add_up(x, high);
     }
     next();
@@ -280,9 +283,14 @@ beam_slices_kernel(const float* logits, long long ld, int vocab, const float* sc
     } else {
         // the few chunks of a thread in which something reaches t are read once more, a thread a vector
         for (int c = 0, v = v0; v < v1; ++c, v += CHUNK)
-            if (chunk_top[c][tid] >= tf) again[atomicAdd(&cell, 1)] = (unsigned short)(c * ST + tid);
+            if (__bfloat162float(tops[c][tid]) >= tf) {
+                const int to = atomicAdd(&cell, 1);
+                if (to < AGAIN) again[to] = (unsigned short)(c * ST + tid);
+            }
         __syncthreads();
-        const int vectors = cell * NV;
+        const bool fits = cell <= AGAIN;                   // else more elements than the gathering has room for
+        if (!fits && tid == 0) listed = CAP + 1;
+        const int vectors = fits ? cell * NV : 0;
         constexpr int AT_ONCE = 2;                         // vectors in flight together
         for (int i0 = tid; i0 < vectors; i0 += AT_ONCE * ST) {
             float y[AT_ONCE][4];
@@ -320,7 +328,9 @@ beam_slices_kernel(const float* logits, long long ld, int vocab, const float* sc
     double total = 0.0;
     {
         const float to = whole_ref(m);                     // (the threads' largest ref, where that is taken)
-        const float ws = warp_sum(sum * two_to(ref - to));
+        double ws = sum * (double)two_to(ref - to);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
         if (lane == 0) wsum[warp] = ws;
     }
     if (__syncthreads_or(sum != sum) || by_difference(m)) {
@@ -339,7 +349,7 @@ beam_slices_kernel(const float* logits, long long ld, int vocab, const float* sc
     }
     if (tid == 0)
 #pragma unroll
-        for (int w = 0; w < W; ++w) total += (double)wsum[w];
+        for (int w = 0; w < W; ++w) total += wsum[w];
 
     int n = listed;
     if (n > CAP) {
@@ -599,15 +609,19 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
 
 int vectors_of(int vocab) { return (vocab + 3) / 4; }
 
-// Slices a row: what takes the fewest rounds of chunks, all CTAs at work, a slice's end costing about what two chunks' way does
+// Slices a row, by about how many us they take: a chunk 0.65 on its way to a CTA, 0.4 of an SM's bandwidth; a slice's end 2, and 1 more for every
+// CTA of the SM, since they come to it together.  (us for 2 / 3 / 4 slices: 512 rows of 128,256 64.0 / 65.9 / 67.2, 128 rows 25.5 / 27.6 / 29.1, 128
+// rows of 50,021 16.9 / 17.4 / 18.3; 4 rows of 128,256 for 8 / 16 / 32 slices 9.5 / 8.9 / 8.8)
 int slices_of(int rows, int vocab, int sms) {
     const int n = vectors_of(vocab), chunks = (n + NV * ST - 1) / (NV * ST);
     int best = chunks;
-    long long best_cost = -1;
+    double best_cost = -1.;
     for (int s = (chunks + MAX_CHUNKS - 1) / MAX_CHUNKS; s <= chunks; s = s < 64 ? s + 1 : 2 * s) {
         const int a_slice = (n + s - 1) / s, of_slice = (a_slice + NV * ST - 1) / (NV * ST);
-        const long long rounds = ((long long)rows * s + CTAS * sms - 1) / (CTAS * sms), cost = rounds * (of_slice + 2);
-        if (of_slice <= MAX_CHUNKS && (best_cost < 0 || cost < best_cost)) { best = s; best_cost = cost; }
+        const double an_sm = (double)rows * s / sms, rounds = an_sm > CTAS ? an_sm / CTAS : 1.;
+        const double way = 0.65 * of_slice * rounds, stream = 0.4 * of_slice * an_sm;
+        const double cost = (way > stream ? way : stream) + rounds * (2. + (an_sm < CTAS ? an_sm : CTAS));
+        if (of_slice <= MAX_CHUNKS && (best_cost < 0. || cost < best_cost)) { best = s; best_cost = cost; }
     }
     return best;
 }
