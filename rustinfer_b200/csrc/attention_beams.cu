@@ -45,8 +45,9 @@ constexpr unsigned SPIN_LIMIT = 1u << 20;
 
 constexpr int KT = 64;                                     // keys of a tile
 constexpr int STAGES = 2;
-// (8 x 8 beams, heads of 64, us behind 4,096 / 16,384 keys: 4 warps, 4 CTAs an SM 28 / 69; 8 warps, 2 CTAs, tiles of 128, 3 stages 28 / 79;
-// 4 warps and 3 CTAs 32 / 83, 5 CTAs 31 / 76.  Heads of 128, 4 x 16 beams behind 12,000: 4 warps, 2 CTAs 84; 8 warps, 2 CTAs 89)
+// (us.  8 x 8 beams, heads of 64, behind 4,096 / 16,384 keys, before a range's start and end took 3 us less: 4 warps, 4 CTAs an SM 28 / 69; 8 warps,
+// 2 CTAs, tiles of 128, 3 stages 28 / 79; 4 warps and 3 CTAs 32 / 83, 5 CTAs 31 / 76.  4 x 16 beams, heads of 128, behind up to 9,001 / 36,004:
+// 4 warps, 2 CTAs 52 / 141; 8 warps, 2 CTAs 59 / 145)
 // rows of shared keys are split over RTILES warps, a tile's keys over the others
 template <int RTILES> constexpr int key_groups() { return WARPS / RTILES < KT / 16 ? WARPS / RTILES : KT / 16; }
 
@@ -159,6 +160,7 @@ template <int RTILES, bool TMA>
 __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, unsigned char* smem, int g, int kvh, int m0, int m_count, const int* bt,
                                        int lo, int hi, int part) {
     constexpr int KG = key_groups<RTILES>();
+    static_assert(RTILES * KG == WARPS, "a warp without a part would read queries that are not there");
     constexpr int WK = KT / KG;                            // keys a warp takes of a tile
     constexpr int NK = WK / 8;
     constexpr int PIECES = (KT * CH + THREADS - 1) / THREADS;      // 16-byte pieces of a tile's keys a thread fetches

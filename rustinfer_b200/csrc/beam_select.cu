@@ -20,7 +20,7 @@
 // The second kernel does the same with 64-bit scores.
 //
 // Scores and the sums over slices are 64-bit: the rows of a group compete through the sums, and a choice hangs on
-// differences however small.  Weights are 32-bit exponentials, summed in 32 bits over a warp's elements and in 64 from there.
+// differences however small.  Weights are 32-bit exponentials, summed in 32 bits over a thread's sixteen of a chunk and in 64 from there.
 #include "common.cuh"
 
 namespace {

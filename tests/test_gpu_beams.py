@@ -111,6 +111,28 @@ def test_choice_among_equals_and_masks(K, kind, vocab):
     _agree(_select(K, logits, scores, beams, picks), _best(logits.cpu().numpy(), scores.cpu().numpy(), beams, picks), vocab)
 
 
+@pytest.mark.parametrize("kind", ["random", "equal", "two values", "one group of equals", "mostly forbidden", "large"])
+def test_choice_from_long_slices(K, kind):
+    """So many rows that a slice is a whole row of thirteen chunks; the rows start at every offset from a 16-byte boundary."""
+    beams, groups, vocab, picks = 4, 50, 50021, 24
+    g = torch.Generator(device="cuda").manual_seed(len(kind))
+    logits = torch.randn((groups * beams, vocab), generator=g, device="cuda")
+    scores = -5 * torch.rand(groups * beams, generator=g, device="cuda")
+    if kind == "equal":
+        logits.fill_(-2.5)
+    elif kind == "two values":                             # half of all words reach any threshold
+        logits = torch.where(logits > 0, 1.0, 0.0)
+    elif kind == "one group of equals":
+        logits[8:12] = 0.5
+        scores[8:12] = -1.0
+    elif kind == "mostly forbidden":
+        logits.masked_fill_(torch.rand(logits.shape, generator=g, device="cuda") > 20 / vocab, -math.inf)
+        logits[5] = -math.inf
+    elif kind == "large":                                  # weights by differences
+        logits[::3] *= 1e6
+    _agree(_select(K, logits, scores, beams, picks), _best(logits.cpu().numpy(), scores.cpu().numpy(), beams, picks), vocab)
+
+
 def test_choice_with_infinite_logits(K):
     logits = torch.randn((2, 9000), device="cuda")
     logits[0, [17, 8000]] = math.inf
