@@ -58,6 +58,7 @@ struct SliceStat {
 };
 __device__ __forceinline__ bool by_difference(float m) { return !(fabsf(m) <= 65536.f); }      // beyond, x L - ref is not near enough
 __device__ __forceinline__ float whole_ref(float m) { return ceilf(m * L); }
+constexpr float LEAST_REF = -131072.f;                     // below whole_ref(-65536) = -94548
 __device__ __forceinline__ float two_to(float whole) {     // 2^whole for a whole number up to 0, exactly; 0 below the normal numbers
     return whole < -126.f ? 0.f : __int_as_float((127 + (int)whole) << 23);
 }
@@ -200,9 +201,10 @@ beam_slices_kernel(const float* logits, long long ld, int vocab, const float* sc
     }
     // A thread's sum of 2^(x L - ref), L = log2 e in 32 bits, ref a whole number that is at least the thread's largest x L: one fused
     // multiply-add an element, whose own rounding is all that is lost, and moving on to another ref is exact.  A chunk's sixteen are
-    // added up in 32 bits, the rest in 64.
+    // added up in 32 bits, the rest in 64.  A ref starts below every one that a slice summed so can have (whole_ref(m) > LEAST_REF): words masked by
+    // large finite numbers weigh nothing beside it, where a ref of their own, rounded by more than the exponents' range, would give them any weight.
     double sum = 0.0;
-    float ref = -1e30f, top = -INFINITY;                   // (top: what is no number does not count)
+    float ref = LEAST_REF, top = -INFINITY;                // (top: what is no number does not count)
     auto add_up = [&](const float (&x)[4 * NV], float high) {
         const float to = fmaxf(ref, ceilf(high * L));
         float part[4] = {0.f, 0.f, 0.f, 0.f};
