@@ -336,15 +336,16 @@ beam_slices_kernel(const float* logits, long long ld, int vocab, const float* sc
         if (lane == 0) wsum[warp] = ws;
     }
     if (__syncthreads_or(sum != sum) || by_difference(m)) {
-        // something is no number, or infinite, or very large: once more
-        float s = 0.f;
+        // something is no number, or infinite, or very large: once more, in 64 bits from element to element
+        double s = 0.0;
         if (m > -INFINITY)
             for (int e = e_lo + tid; e < e_hi; e += ST) {
                 const float v = fmaxf(row[e], -INFINITY);
-                s += m == INFINITY ? (v == INFINITY ? 1.f : 0.f)   // the weight lies on the infinite ones alone
-                                   : ex2(by_difference(m) ? (v - m) * L : fmaf(v, L, -whole_ref(m)));
+                s += (double)(m == INFINITY ? (v == INFINITY ? 1.f : 0.f)   // the weight lies on the infinite ones alone
+                                            : ex2(by_difference(m) ? (v - m) * L : fmaf(v, L, -whole_ref(m))));
             }
-        s = warp_sum(s);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         __syncthreads();
         if (lane == 0) wsum[warp] = s;
         __syncthreads();
