@@ -456,7 +456,8 @@ beam_merge_kernel(const unsigned long long* best, const SliceStat* stat, const f
             } else if (by_difference(s.m)) {
                 sum += s.m == m ? s.sum : s.sum * exp((double)s.m - (double)m);
             } else {
-                sum += s.sum * exp(0.6931471805599453 * whole_ref(s.m) - (double)m);
+                // (that L is not log2 e to the last bit is made up for by the slice's largest logit: of 65,536 it is 9e-4 of the weight)
+                sum += s.sum * exp(0.6931471805599453 * whole_ref(s.m) + (double)s.m * (1.0 - 0.6931471805599453 * (double)L) - (double)m);
             }
         }
 #pragma unroll

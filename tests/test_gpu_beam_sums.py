@@ -28,3 +28,16 @@ def test_sums_of_long_flat_rows(K, what):  # noqa: F811
     got, want = _select(K, logits, scores, 1, picks), _best(logits.cpu().numpy(), scores.cpu().numpy(), 1, picks)
     _agree(got, want, vocab)
     assert (abs(got[0] - want[0]) <= 2.0 ** -24 * abs(want[0]) + 10 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("top", [65537.0, 65540.0, 65600.0])
+def test_rows_with_slices_on_both_sides_of_what_is_large(K, top):  # noqa: F811
+    """Weights are summed by differences in the slices whose largest logit is beyond 65,536 and by powers of two in the others; a row's
+    continuations hang on both."""
+    vocab = 40000
+    logits = torch.full((6, vocab), -100.0, device="cuda")
+    for r in range(6):
+        logits[r, 5 + r] = top
+        logits[r, 39000 - 5000 * r] = 65536.0 - r / 128
+    scores = torch.zeros(6, device="cuda")
+    _agree(_select(K, logits, scores, 3, 6), _best(logits.cpu().numpy(), scores.cpu().numpy(), 3, 6), vocab)
