@@ -40,7 +40,6 @@ constexpr int OWN_KEYS = 16;                               // keys of its own a 
 constexpr int OWN_STAGES = 2;                              // of which so many are on their way
 constexpr bool BY_TMA = HD == 64 || HD == 128;
 constexpr int TKB_OR_1 = BY_TMA ? HD / 64 : 1;             // 64-column blocks of a head
-constexpr int NO_KEY = (int)0x80000000;                    // in place of a page
 constexpr unsigned SPIN_LIMIT = 1u << 20;
 
 constexpr int KT = 64;                                     // keys of a tile
@@ -208,13 +207,14 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
     const bool small_pages = a.page_size < KT;             // a page a box; else a tile lies in one page
     const int box_row = (box_kv * a.Hkv + kvh) * a.page_size, page_rows = 2 * a.Hkv * a.page_size;
     const unsigned box_at = ((box_kv * TKB_OR_1 + box_kb) * KT + box_c * a.box_rows) * 128;
-    int next_page = NO_KEY, next_off = 0;                  // of the tile that was looked up (nothing waits for the load before the fetch does)
+    int next_page = 0, next_off = 0;                       // of the tile that was looked up (nothing waits for the load before the fetch does)
+    bool next_box = false;
     int blk = small_pages ? t0 * boxes : t0 * KT / a.page_size, off = small_pages ? 0 : t0 * KT % a.page_size;
     auto look_up_box = [&](int t) {                        // tiles in order
         const int key = (t0 + t) * KT + box_c * a.box_rows;
-        next_page = NO_KEY;                                // boxes without a key in [lo, hi) are not fetched
+        next_box = box_kv < 2 && key < hi && key + a.box_rows > lo;        // boxes without a key in [lo, hi) are not fetched
         next_off = off;
-        if (box_kv < 2 && key < hi && key + a.box_rows > lo) next_page = bt[blk + (small_pages ? box_c : 0)];
+        if (next_box) next_page = bt[blk + (small_pages ? box_c : 0)];
         if (small_pages) blk += boxes;
         else if ((off += KT) >= a.page_size) { off = 0; ++blk; }
     };
@@ -222,7 +222,7 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
         if constexpr (TMA) {
             if (warp == 0) {
                 const int page = (unsigned)next_page > (unsigned)a.pages ? a.pages : next_page;      // outside the cache: rows behind the matrix, zeros
-                const bool mine = next_page != NO_KEY;
+                const bool mine = next_box;
                 const unsigned all = __ballot_sync(0xffffffffu, mine);
                 if (lane == 0) bar_expect(&full[stage], (unsigned)__popc(all) * a.box_rows * 128);
                 __syncwarp();

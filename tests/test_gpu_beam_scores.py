@@ -1,0 +1,32 @@
+"""The attention of beams where a shared page has the lowest number there is."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_beams import K, _attention, _beams, _near  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 8), (128, 64), (64, 5), (48, 16)])
+@pytest.mark.parametrize("bad", [-(1 << 31), -(1 << 31) + 1, (1 << 31) - 1])
+def test_shared_pages_of_the_numbers_at_the_ends(K, dim, page, bad):  # noqa: F811
+    """A page of zeros in a group's shared keys, whatever the number outside the cache; what the stages held before is no number."""
+    heads, kv_heads, beams = 4, 2, 3
+    q, cache, table, kv_len, sh = _beams(2, beams, heads, kv_heads, dim, page, [310, 200], [[40, 33, 21], [5, 1, 30]], seed=dim + page)
+    zeros = int((set(range(cache.shape[0])) - set(table[table >= 0].tolist())).pop())
+    cache[zeros] = 0
+    table[:3, 64 // page + 1] = bad
+    table[:3, 200 // page] = bad
+    table[3:, 0] = bad
+    used = torch.arange(table.shape[1], device="cuda")[None] * page < kv_len[:, None]
+    want_table = torch.where((table < 0) | (table >= cache.shape[0]), zeros, table)
+    want = _attention(q, cache, want_table, kv_len, heads, kv_heads, dim, 0.125, None)
+    out = torch.empty_like(q)
+    for hints in ((310, 40), (1, 1)):                      # ranges of a tile or two, and one of all tiles
+        # CTAs whose stages hold no numbers, then the call
+        nan = torch.full_like(cache, math.nan)
+        K.attention_decode_beams(q, out, nan, table.clamp(min=0, max=cache.shape[0] - 1), kv_len, sh, beams, heads, kv_heads, dim, 0.125, None, 310, 40)
+        K.attention_decode_beams(q, out, cache, torch.where(used, table, 0), kv_len, sh, beams, heads, kv_heads, dim, 0.125, None, *hints)
+        _near(out, *want, dim, 360)
