@@ -41,6 +41,9 @@ constexpr int OWN_STAGES = 2;                              // of which so many a
 constexpr bool BY_TMA = HD == 64 || HD == 128;
 constexpr int TKB_OR_1 = BY_TMA ? HD / 64 : 1;             // 64-column blocks of a head
 constexpr unsigned SPIN_LIMIT = 1u << 20;
+// A weight is 2^(fma(score, scale, -maximum)), which leaves out the rounding that the maximum, a product itself, has had.  That is a factor of a
+// tile's weights, and next to nothing, until it passes the exponents' range: beyond FAR the scores are rounded first, and the largest weight is 1.
+constexpr float FAR = 16777216.f;
 
 constexpr int KT = 64;                                     // keys of a tile
 constexpr int STAGES = 2;
@@ -344,7 +347,7 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
         for (int n = 0; n < NK; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
-        float alpha[2], muse[2];
+        float alpha[2], muse[2], by[2] = {a.scale_log2, a.scale_log2};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
@@ -354,6 +357,14 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
             alpha[i] = ex2(m[i] - muse[i]);
             m[i] = mnew;
             l[i] *= alpha[i];
+            if (fabsf(muse[i]) > FAR) {                    // rounded ahead of the subtraction
+#pragma unroll
+                for (int n = 0; n < NK; ++n) {
+                    s[n][2 * i] = __fmul_rn(s[n][2 * i], a.scale_log2);
+                    s[n][2 * i + 1] = __fmul_rn(s[n][2 * i + 1], a.scale_log2);
+                }
+                by[i] = 1.f;
+            }
         }
         if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
@@ -366,7 +377,7 @@ __device__ __forceinline__ void attend(const Args& a, const CUtensorMap* map, un
         for (int n = 0; n < NK; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                s[n][e] = ex2(fmaf(s[n][e], a.scale_log2, -muse[e >> 1]));
+                s[n][e] = ex2(fmaf(s[n][e], by[e >> 1], -muse[e >> 1]));
                 l[e >> 1] += s[n][e];
             }
 #pragma unroll
@@ -536,11 +547,12 @@ __device__ __forceinline__ void attend_own(const Args& a, unsigned char* smem, i
         l *= alpha;
 #pragma unroll
         for (int n = 0; n < NT; ++n) { o[n][0] *= alpha; o[n][1] *= alpha; }
+        const bool far = fabsf(muse) > FAR;
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                s[n][e] = ex2(fmaf(s[n][e], a.scale_log2, -muse));
+                s[n][e] = ex2(far ? __fmul_rn(s[n][e], a.scale_log2) - muse : fmaf(s[n][e], a.scale_log2, -muse));
                 l += s[n][e];
             }
         unsigned ph[2], pl[2];

@@ -1,4 +1,4 @@
-"""The attention of beams where a shared page has the lowest number there is."""
+"""The attention of beams where a shared page has the lowest number there is, and where the products of queries and keys are huge."""
 import math
 
 import pytest
@@ -30,3 +30,27 @@ def test_shared_pages_of_the_numbers_at_the_ends(K, dim, page, bad):  # noqa: F8
         K.attention_decode_beams(q, out, nan, table.clamp(min=0, max=cache.shape[0] - 1), kv_len, sh, beams, heads, kv_heads, dim, 0.125, None, 310, 40)
         K.attention_decode_beams(q, out, cache, torch.where(used, table, 0), kv_len, sh, beams, heads, kv_heads, dim, 0.125, None, *hints)
         _near(out, *want, dim, 360)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (16, 2, 128), (8, 8, 48)])
+@pytest.mark.parametrize("size", [2.0 ** 4, 2.0 ** 12, 2.0 ** 20, 2.0 ** 26, 2.0 ** 30, -2.0 ** 26])
+def test_products_of_any_size(K, heads, kv_heads, dim, size):  # noqa: F811
+    """Keys that are multiples of one row of signs and queries that are one too, so that every product is a whole number times `size` and is exact;
+    the largest stands `size` * dim * scale >= 16 * 48 / 8 = 96 above the next, whose weight is then below 2^-126: the output is the
+    largest key's value, as it is stored."""
+    beams, shared, mine = 3, [200, 70], [[10, 4, 7], [30, 31, 1]]
+    q, cache, table, kv_len, sh = _beams(2, beams, heads, kv_heads, dim, 16, shared, mine, seed=dim)
+    signs = torch.where(torch.arange(dim, device="cuda") % 3 == 0, -1.0, 1.0)
+    q[:] = (size * signs).repeat(heads).bfloat16()
+    order = torch.randperm(256, generator=torch.Generator(device="cuda").manual_seed(dim), device="cuda").tolist()
+    for i in range(2):                                     # a number of its own for every key of the longest row; the shared ones are alike
+        for r in range(3 * i, 3 * i + 3):
+            for t in range(int(kv_len[r])):
+                cache[int(table[r, t // 16]), 0, :, t % 16] = (order[t] * signs).bfloat16()
+    table = table.clamp(min=0)
+    out = torch.empty_like(q)
+    K.attention_decode_beams(q, out, cache, table, kv_len, sh, beams, heads, kv_heads, dim, 0.125, None, 200, 30)
+    for r, n in enumerate(kv_len.tolist()):
+        t = (max if size > 0 else min)(range(n), key=lambda t: order[t])
+        want = cache[int(table[r, t // 16]), 1, :, t % 16].repeat_interleave(heads // kv_heads, 0).reshape(-1)
+        assert torch.equal(out[r], want), r
