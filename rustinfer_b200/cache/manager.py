@@ -266,16 +266,33 @@ class CacheManager:
             return 0
         return min(min(r.common, r.length) for r in reqs)
 
-    def reorder(self, request_ids: Sequence[Any], parents: Sequence[int]) -> DeviceReorder:
-        """Request r takes over what request parents[r] holds, all at once; any mapping.  The requests are of one family and of
-        equal length.  Full pages change holders; the page that is partly filled and the state slot stay whose they are, and
-        their content moves."""
-        self._no_lease("reorder")
+    def _family(self, request_ids: Sequence[Any], parents: Sequence[int]) -> List[_Request]:
+        """The requests of a reorder that can be; raises before anything is changed."""
         reqs = [self._req[i] for i in request_ids]
         if len(parents) != len(reqs) or any(not 0 <= p < len(reqs) for p in parents) or len(set(request_ids)) != len(reqs):
             raise ValueError(f"reorder: {len(reqs)} requests and the parents {list(parents)!r}")
         if any(r.length != reqs[0].length or r.family != reqs[0].family for r in reqs):
             raise ValueError("reorder: the requests are not of one family and one length")
+        return reqs
+
+    def reorder_families(self, request_ids: Sequence[Any], parents: Sequence[int], beams: int) -> List[DeviceReorder]:
+        """`reorder` of every `beams` requests that follow one another; parents are places in `request_ids`, of the same family.  All
+        or nothing: every family is looked at before any is changed."""
+        n = len(request_ids)
+        if beams < 1 or n % beams or len(parents) != n or len(set(request_ids)) != n:
+            raise ValueError(f"reorder: {list(request_ids)!r} and the parents {list(parents)!r} in families of {beams}")
+        families = [(request_ids[i: i + beams], [p - i for p in parents[i: i + beams]]) for i in range(0, n, beams)]
+        self._no_lease("reorder")
+        for ids, up in families:
+            self._family(ids, up)
+        return [self.reorder(ids, up) for ids, up in families]
+
+    def reorder(self, request_ids: Sequence[Any], parents: Sequence[int]) -> DeviceReorder:
+        """Request r takes over what request parents[r] holds, all at once; any mapping.  The requests are of one family and of
+        equal length.  Full pages change holders; the page that is partly filled and the state slot stay whose they are, and
+        their content moves."""
+        self._no_lease("reorder")
+        reqs = self._family(request_ids, parents)
         full, used = divmod(reqs[0].length, self.page_size) if reqs else (0, 0)
         out = DeviceReorder([int(p) for p in parents], [r.slot for r in reqs], {}, used)
         for g, pool in self.pools.items():

@@ -429,7 +429,8 @@ class ModelRunner:
 
     def reorder(self, request_ids: Sequence[Any], parents: Sequence[int], beams: Optional[int] = None) -> None:
         """Request r takes over what request parents[r] has computed, all at once.  Any mapping among every `beams` requests that
-        follow one another (default: all of them), which are forks of one request and of equal length."""
+        follow one another (default: all of them), which are forks of one request and of equal length; no request twice.  What cannot
+        be is refused before anything is changed."""
         n = len(request_ids)
         k = n if beams is None else int(beams)
         if n == 0 and not len(parents):
@@ -439,7 +440,7 @@ class ModelRunner:
         if all(p == i for i, p in enumerate(parents)):
             return
         self._zero_new_state()
-        moves = [self.cache.reorder(request_ids[i: i + k], [p - i for p in parents[i: i + k]]) for i in range(0, n, k)]
+        moves = self.cache.reorder_families(request_ids, parents, k)
         paged = self.layout.paged_groups()
         slots = [s for m in moves for s in m.slots]
         tokens = [m.tokens for m in moves for _ in m.slots]
