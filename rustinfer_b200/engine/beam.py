@@ -10,6 +10,7 @@ options follow its sampling parameters where they mean the same (crates/infer-co
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 from typing import Any, Dict, List, Optional, Sequence, Tuple
 
@@ -37,6 +38,8 @@ class BeamParams:
             raise ValueError("max_tokens must be at least 1")
         if not self.length_penalty == self.length_penalty or abs(self.length_penalty) == float("inf"):
             raise ValueError("length_penalty must be finite")
+        if abs(self.length_penalty) * math.log(self.max_tokens) > 600.0:       # e ** 600: a factor e ** 109 inside what 64 bits hold
+            raise ValueError(f"length_penalty {self.length_penalty}: {self.max_tokens} tokens ** length_penalty leaves the range of 64 bits")
 
 
 @dataclass
