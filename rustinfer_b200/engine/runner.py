@@ -597,11 +597,11 @@ class ModelRunner:
         that the next step overwrites (for callers that consume it at once).
 
         `beams` above 1: the entries are single tokens, and every `beams` of them that follow one another are forks of
-        one request (`fork`), whose common keys are read once where there are many (`beam_keys`)."""
+        one request (`fork`), whose common keys are read once where there are many (`beam_keys`) and no more than 64 beams."""
         ids = self._validate(entries)
         if beams > 1 and (len(entries) % beams or any(len(e.tokens) != 1 for e in entries)):
             raise StepError(f"{len(entries)} entries are no single tokens of {beams} beams a request")
-        if beams > 1 and beams * sum(self._common(entries, beams)) < self.beam_keys:
+        if beams > _k.BEAMS_MAX or (beams > 1 and beams * sum(self._common(entries, beams)) < self.beam_keys):
             beams = 0
         lease = self.cache.lease([(e.request_id, len(e.tokens)) for e in entries])
         try:

@@ -143,3 +143,21 @@ def test_requests_of_several_families_share_nothing(folder, calls):
         held.add(i, n)
     _step_and_check(r, held, calls, saved, ["a", "b", "c", "d"], 2, 5, [0, 0])
     _step_and_check(r, held, calls, saved, ["a", "b", "c", "d"], 4, 6, [0])
+
+
+@pytest.mark.parametrize("sizes", [[], [66]])
+def test_more_beams_than_are_read_together(folder, calls, sizes):
+    """More than 64 forks of one request in a step are read row by row; the logits are those of steps of 33 and 33, to the bound that the ways
+    of decoding are held to elsewhere (6e-2 of the largest logit)."""
+    from rustinfer_b200.engine.runner import StepEntry
+    r = _runner(folder("D"), max_batch_seqs=140, num_pages=400, capture_sizes=sizes)
+    prompt = random_ids(40, r.spec.vocab_size, 1)
+    r.open(0)
+    r.step([StepEntry(0, prompt, [0])])
+    r.fork(0, list(range(1, 132)))
+    new = random_ids(66, r.spec.vocab_size, 2)
+    x = r.step([StepEntry(i, [t], [0]) for i, t in enumerate(new)], beams=66).clone()
+    assert not calls
+    y = r.step([StepEntry(66 + i, [t], [0]) for i, t in enumerate(new)], beams=33)
+    assert calls
+    assert float((x - y).abs().max()) <= 6e-2 * float(y.abs().max())
