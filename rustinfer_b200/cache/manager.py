@@ -260,7 +260,8 @@ class CacheManager:
         return copies
 
     def common_length(self, request_ids: Sequence[Any]) -> int:
-        """Tokens at the start that these requests certainly share (0 for requests of several families)."""
+        """Tokens at the start that these requests certainly share (0 for requests of several families): what their family had when it was forked.
+        What a reorder makes them share behind that is not counted."""
         reqs = [self._req[i] for i in request_ids]
         if any(r.family != reqs[0].family for r in reqs):
             return 0

@@ -26,7 +26,7 @@ class BeamParams:
     best: int = 1                       # of them returned, best first
     max_tokens: int = 16
     length_penalty: float = 1.0         # a hypothesis counts as log-probability / tokens ** length_penalty
-    early_stopping: bool = False        # True: a prompt is done when `beams` hypotheses have ended
+    early_stopping: bool = False        # True: a prompt is done when `beams` hypotheses have ended; else when no live beam, as long as it is, is worth more
     ignore_eos: bool = False
 
     def validate(self) -> None:
@@ -113,7 +113,8 @@ class _Search:
                     self.end(t, s, p, "length")
             over = True
         if len(self.ended) >= p.beams and not over:
-            # no live beam can come to more than the best has now, by its length now
+            # the usual rule: no live beam, counted by its length now, comes to more than the worst that has ended (with a length_penalty above 0 one
+            # that grew longer still could)
             over = p.early_stopping or self.ended[-1].score >= best / made ** p.length_penalty
         return parents, over
 

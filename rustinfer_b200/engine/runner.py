@@ -268,7 +268,8 @@ class ModelRunner:
 
     # Steps of beams read their requests' common keys once when all beams together see at least so many of them: below, the rows' own
     # kernel, whose later rows find them in L2, is sooner (us a layer of 8 key heads of 64, rows / beams: 64 rows behind 300 keys 9 / 13,
-    # behind 1,000 18 / 17, behind 4,000 61 / 26; 8 rows behind 4,000 14 / 15)
+    # behind 1,000 18 / 17, behind 4,000 61 / 26; 8 rows behind 4,000 14 / 15).  One number, from this one geometry: head sizes, key heads and
+    # windows do not enter
     beam_keys = 64 * 1024
 
     def __init__(self, model_dir: str, dtype="bfloat16", device="cuda:0", max_model_len: int = 4096,
@@ -468,7 +469,7 @@ class ModelRunner:
 
     # --------------------------------------------------------------------------- plan
     def _common(self, entries: Sequence[StepEntry], beams: int) -> List[int]:
-        """Keys that the requests of every `beams` entries have in common."""
+        """Keys that the requests of every `beams` entries have in common, as far as they were when they were forked."""
         return [self.cache.common_length([e.request_id for e in entries[i: i + beams]]) for i in range(0, len(entries), beams)]
 
     def _validate(self, entries: Sequence[StepEntry]) -> Optional[np.ndarray]:
