@@ -2056,7 +2056,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, out_scor
 
     logits fp32 [groups * beams, vocab] (unit column stride, any row stride), scores fp32 [groups * beams].  The outputs
     [groups, picks] get, best first, the scores (fp32), the rows they continue (int32, counted over all groups) and the
-    tokens (int32).  Equal scores go by ascending (row, token); scores are compared in 64 bits.  A running score is finite
+    tokens (int32).  Equal scores go by ascending (row, token); scores are compared in 64 bits (of one row's words whose logits differ by
+    less than those bits tell, which takes logits below 1e-7 in size, some go by their logits).  A running score is finite
     or -inf; a row whose score is -inf or not a number has no continuation but of score -inf, and neither has a token whose
     logit is -inf or not a number.  In a row that holds +inf, those tokens share the weight.  Up to 64 beams and 128 picks."""
     _here("beam_select", logits, scores, out_scores, out_rows, out_tokens)
@@ -2193,7 +2194,8 @@ def attention_decode_beams(q: torch.Tensor, out: torch.Tensor, cache: torch.Tens
     without keys gets zeros; a page number outside the cache stands for a page of zeros.  A group one of whose rows has fewer keys than shared_len, or whose rows' windows start at different
     keys, is read row by row.  most_shared and most_own: about how many keys the longest shared part and the longest rest have
     (they choose how the work is cut, not what is computed).  part_o, part_lse: fp32 scratch (`decode_scratch_floats` with the
-    sum of `attention_beams_splits`, at most BEAM_SPLITS_MAX); without them it is allocated."""
+    sum of `attention_beams_splits`, at most BEAM_SPLITS_MAX); without them it is allocated.  The first call on a device is not
+    captured."""
     _here("attention_decode_beams", q, out, cache, block_table, kv_len, shared_len, part_o, part_lse)
     R, width = q.shape[0], num_heads * head_dim
     entry, shared, own, ctas, need_o, need_l = _attention_beams_plan(R, beams, num_heads, num_kv_heads, head_dim, max(0, int(most_shared if window is None else min(most_shared, window + 64))), max(1, int(most_own)),
@@ -2217,6 +2219,8 @@ def attention_decode_beams(q: torch.Tensor, out: torch.Tensor, cache: torch.Tens
         raise KernelError(f"attention_decode_beams: a window of {window} keys, a scale of {scale}")
     if R == 0:
         return
+    if q.device not in _tc_state and torch.cuda.is_current_stream_capturing():
+        raise KernelError("attention_decode_beams: the first call on a device makes what the kernels share there; make one ahead of the capture")
     if part_o is None or part_lse is None:
         scratch = torch.empty(need_o + need_l, dtype=torch.float32, device=q.device)
         o_ptr = scratch.data_ptr()
