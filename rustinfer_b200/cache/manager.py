@@ -284,16 +284,17 @@ class CacheManager:
             raise ValueError(f"reorder: {list(request_ids)!r} and the parents {list(parents)!r} in families of {beams}")
         families = [(request_ids[i: i + beams], [p - i for p in parents[i: i + beams]]) for i in range(0, n, beams)]
         self._no_lease("reorder")
-        for ids, up in families:
-            self._family(ids, up)
-        return [self.reorder(ids, up) for ids, up in families]
+        looked_at = [(self._family(ids, up), up) for ids, up in families]
+        return [self._reorder(reqs, up) for reqs, up in looked_at]
 
     def reorder(self, request_ids: Sequence[Any], parents: Sequence[int]) -> DeviceReorder:
         """Request r takes over what request parents[r] holds, all at once; any mapping.  The requests are of one family and of
         equal length.  Full pages change holders; the page that is partly filled and the state slot stay whose they are, and
         their content moves."""
         self._no_lease("reorder")
-        reqs = self._family(request_ids, parents)
+        return self._reorder(self._family(request_ids, parents), parents)
+
+    def _reorder(self, reqs: List[_Request], parents: Sequence[int]) -> DeviceReorder:
         full, used = divmod(reqs[0].length, self.page_size) if reqs else (0, 0)
         out = DeviceReorder([int(p) for p in parents], [r.slot for r in reqs], {}, used)
         for g, pool in self.pools.items():
