@@ -99,6 +99,11 @@ class _DecodeGraph:
     of page 0 and writes nothing (RustInfer pads with one-token rows on a scratch block,
     crates/infer-worker/src/application/worker_scheduler.rs:685-718)."""
 
+    # own keys a beam that a step of beams is cut for: two ranges.  (us a layer against row by row, for cuts of 64 / 200 / 400, heads of 64: 8 x 8 beams
+    # behind 4,000 keys, 10 own ones -27 / -26 / -27, 300 -5 / -14 / -21, 600 +22 / 0 / -13; 4 x 16 behind 16,000, 10 own -158 / -158 / -144, 1,000
+    # -107 / -146 / -152)
+    OWN_KEYS = 200
+
     def __init__(self, runner: "ModelRunner", bucket: int, beams: int = 0):
         self.bucket = bucket
         self.beams = beams
@@ -162,7 +167,7 @@ class _DecodeGraph:
             num_tokens=bucket, num_entries=bucket, token_ids=v[0], positions=v[1], cu_q=v[2], kv_len=v[3],
             state_slots=v[4], groups=gsteps, entries=[], max_q_len=1,
             max_kv_len=runner.max_model_len, decode_only=True, indices=indices,
-            beams=beams, shared_len=v[-1] if beams > 1 else None, max_own_len=min(64, runner.max_model_len) if beams > 1 else 0)
+            beams=beams, shared_len=v[-1] if beams > 1 else None, max_own_len=min(self.OWN_KEYS, runner.max_model_len) if beams > 1 else 0)
         self.rows = v[5]
         # one eager run (libraries pick their algorithms, lazy kernels get built), then capture
         torch.cuda.synchronize()
@@ -266,11 +271,9 @@ class _DecodeGraph:
 class ModelRunner:
     """Model, cache and step function of one model folder on one GPU."""
 
-    # Steps of beams read their requests' common keys once when all beams together see at least so many of them: below, the rows' own
-    # kernel, whose later rows find them in L2, is sooner (us a layer of 8 key heads of 64, rows / beams: 64 rows behind 300 keys 9 / 13,
-    # behind 1,000 18 / 17, behind 4,000 61 / 26; 8 rows behind 4,000 14 / 15).  One number, from this one geometry: head sizes, key heads and
-    # windows do not enter
-    beam_keys = 64 * 1024
+    # Steps of beams read their requests' common keys together where that takes no longer (`attention_beams_sooner`); with a number here, where all
+    # beams together see at least so many of them.  (Keys that a window hides are counted: no model with windows takes the kernel.)
+    beam_keys: Optional[int] = None
 
     def __init__(self, model_dir: str, dtype="bfloat16", device="cuda:0", max_model_len: int = 4096,
                  page_size: int = 16, num_pages: Optional[int] = None, max_batch_seqs: int = 64,
@@ -327,6 +330,9 @@ class ModelRunner:
         self.steps_run = 0
         self.h2d_bytes_last = 0
         self.graph_replays = 0
+        # (heads, key heads, head size) of the largest mixer that can read beams together
+        self._beam_sizes = max(((m.Hq, m.Hkv, m.hd) for m in (b.mixer for b in self.model.blocks) if getattr(m, "use_mma", False)),
+                               key=lambda s: s[1] * s[2], default=None)
         self._graphs: Dict[Any, "_DecodeGraph"] = {}          # by rows; by (rows, beams a request) of steps of beams
         self._graph_pool = None
         self.use_graphs = bool(self.capture_sizes) and self.model.graph_safe
@@ -472,6 +478,19 @@ class ModelRunner:
         """Keys that the requests of every `beams` entries have in common, as far as they were when they were forked."""
         return [self.cache.common_length([e.request_id for e in entries[i: i + beams]]) for i in range(0, len(entries), beams)]
 
+    def _together(self, entries: Sequence[StepEntry], beams: int) -> bool:
+        """Whether a step of beams reads its requests' common keys once for all of a request's beams, or row by row."""
+        if beams > _k.BEAMS_MAX:
+            return False
+        common = self._common(entries, beams)
+        keys = beams * sum(common)
+        if self.beam_keys is not None:
+            return keys >= self.beam_keys
+        if not self._beam_sizes:
+            return False
+        own = max(self.cache.length(e.request_id) + 1 - c for e, c in zip(entries[::beams], common))
+        return _k.attention_beams_sooner(len(entries), beams, *self._beam_sizes, keys, own)
+
     def _validate(self, entries: Sequence[StepEntry]) -> Optional[np.ndarray]:
         """Raises `StepError` for a step that cannot be; returns the ids of a step of many tokens as one array (None: as they are)."""
         if not entries:
@@ -598,11 +617,11 @@ class ModelRunner:
         that the next step overwrites (for callers that consume it at once).
 
         `beams` above 1: the entries are single tokens, and every `beams` of them that follow one another are forks of
-        one request (`fork`), whose common keys are read once where there are many (`beam_keys`) and no more than 64 beams."""
+        one request (`fork`), whose common keys are read once where that is sooner (`beam_keys`) and no more than 64 beams."""
         ids = self._validate(entries)
         if beams > 1 and (len(entries) % beams or any(len(e.tokens) != 1 for e in entries)):
             raise StepError(f"{len(entries)} entries are no single tokens of {beams} beams a request")
-        if beams > _k.BEAMS_MAX or (beams > 1 and beams * sum(self._common(entries, beams)) < self.beam_keys):
+        if beams > 1 and not self._together(entries, beams):
             beams = 0
         lease = self.cache.lease([(e.request_id, len(e.tokens)) for e in entries])
         try:

@@ -2146,6 +2146,32 @@ def attention_beams_supports(num_heads: int, num_kv_heads: int, head_dim: int) -
     return num_kv_heads > 0 and num_heads % num_kv_heads == 0 and head_dim % 16 == 0 and 16 <= head_dim <= L.MMA_MAX_HEAD_DIM
 
 
+def attention_beams_sooner(rows: int, beams: int, num_heads: int, num_kv_heads: int, head_dim: int, keys: int, own: int) -> bool:
+    """Whether a layer of a captured step of beams takes no longer with the common keys read together than row by row.  keys: common ones that
+    all rows together see; own: of the longest rest.
+
+    What is saved goes by the common keys' bytes, and pays for the second kernel from 64,000 keys of 8 heads of 128 on; of two beams half is saved, so
+    it takes half as many more.  A row's own keys are walked by a warp a range: 480 of them cost what 64,000 save; steps of more than 32 rows with
+    heads above 64 have a start of 512.  With few rows a request's walk, 16 ranges at most, is longer than what all rows read.
+    (us a layer of a captured step, the products in it, row by row / together, requests x beams behind common + own keys of 8 key heads.  32 heads of 64:
+    4 x 4 behind 8,273 + 60 114 / 104, + 400 115 / 115; 8 x 8 behind 1,536 + 60 108 / 109, behind 4,116 + 150 144 / 120, behind 4,000 + 1,000 155 / 171,
+    behind 16,000 + 1,000 320 / 197; 1 x 4 behind 33,095 + 10 101 / 113, 2 x 4 behind 16,547 + 60 101 / 99; 16 x 2 behind 8,232 + 150 137 / 128.  32
+    heads of 128: 4 x 8 behind 1,024 + 60 164 / 168, behind 2,068 + 60 180 / 171, + 400 186 / 194, behind 4,116 + 400 215 / 201; 16 x 4 behind 1,034 + 400
+    233 / 218, behind 1,000 + 1,000 249 / 256.  Over 1,396 such steps what is chosen takes 4 % longer at most, 24 x 2 behind 5,488 + 60 140 / 145.)"""
+    tiles = _beam_row_tiles(beams * (num_heads // num_kv_heads))
+    size = num_kv_heads * head_dim
+    if rows * size <= 1900 + 1500 * tiles:
+        return False
+    many = rows > 32 and head_dim > 64
+    need = (64000 << 10) / size * (1.5 if beams == 2 and not many else 1.0)
+    return keys >= need and own <= 100 + 480 * (keys / need - 1) + (512 if many else 0)
+
+
+def _beam_row_tiles(rows: int) -> int:
+    """As `ri_attention_beams_row_tiles`, without the library."""
+    return 1 if rows <= 16 else 2 if rows <= 32 else 4
+
+
 BEAM_SPLITS_MAX = 20          # ranges of a row's keys at most: 16 of shared ones, 4 of its own
 
 
@@ -2161,7 +2187,7 @@ def _attention_beams_plan(rows: int, beams: int, num_heads: int, num_kv_heads: i
     enough of it for the rows' own keys: by about 6 us and 2 a tile of 64 keys for the former, 3 us and 1 a step of 16 for a row's warp, both
     for heads of 64.  (Over 23 shapes 3 % behind the best cut of each, 9 % at most.  us, against a fixed 6 or 7 eighths with ranges of 32 own
     keys: 4 x 16 beams, heads of 128, of 9,001 and 100 keys 44 and 53, of 2,000 and 300 31 and 36, of 9,001 and 1,000 71 and 84; 8 x 8,
-    heads of 64, of 4,096 and 1,000 52 and 62.  These are calls that say how many own keys there are, as eager steps do; a captured step says 64
+    heads of 64, of 4,096 and 1,000 52 and 62.  These are calls that say how many own keys there are, as eager steps do; a captured step says 200
     for as long as it lives.)"""
     if not attention_beams_supports(num_heads, num_kv_heads, head_dim):
         raise KernelError(f"attention_decode_beams: {num_heads} heads over {num_kv_heads} of {head_dim} (a multiple of 16 up to {L.MMA_MAX_HEAD_DIM})")

@@ -161,3 +161,28 @@ def test_more_beams_than_are_read_together(folder, calls, sizes):
     y = r.step([StepEntry(66 + i, [t], [0]) for i, t in enumerate(new)], beams=33)
     assert calls
     assert float((x - y).abs().max()) <= 6e-2 * float(y.abs().max())
+
+
+def test_steps_take_the_sooner_way(tmp_path):
+    """Without a number in `beam_keys` a step reads together while that is the sooner way: behind enough common keys, until there are too many own
+    ones, from a captured step of its own kind; the 32-bit engine and few rows never."""
+    from rustinfer_b200.engine.runner import StepEntry
+    cfg = dict(helpers.TINY["E"], num_attention_heads=8, num_key_value_heads=8, max_position_embeddings=9000)
+    path = write_random_model(str(tmp_path), cfg, seed=5, std=0.12, norm_std=0.1)
+    for dtype, families, common, together in (("bfloat16", "ab", 8100, True), ("bfloat16", "ab", 7000, False), ("bfloat16", "a", 8100, False),
+                                              ("float32", "ab", 8100, False)):
+        r = _runner(path, dtype=dtype, max_model_len=9000, num_pages=1300, max_batch_tokens=64, capture_sizes=[8])
+        r.beam_keys = None
+        ids = [f + k for f in families for k in "0123"]
+        for f in families:
+            r.open(f + "0")
+            with r.cache.lease([(f + "0", common)]):       # keys of zeros: what they are does not matter
+                pass
+            r.fork(f + "0", [f + k for k in "123"])
+        for own, chosen in ((0, together), (60, together), (500, False)):
+            for i in ids:
+                with r.cache.lease([(i, common + own - r.cache.length(i))]):
+                    pass
+            r._graphs.clear()
+            x = r.step([StepEntry(i, [5], [0]) for i in ids], beams=4)
+            assert bool(x.isfinite().all()) and list(r._graphs) == [(8, 4) if chosen else 8], (dtype, families, common, own)
