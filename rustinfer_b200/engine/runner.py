@@ -99,12 +99,7 @@ class _DecodeGraph:
     of page 0 and writes nothing (RustInfer pads with one-token rows on a scratch block,
     crates/infer-worker/src/application/worker_scheduler.rs:685-718)."""
 
-    # own keys a beam that a step of beams is cut for: two ranges.  (us a layer against row by row, for cuts of 64 / 200 / 400, heads of 64: 8 x 8 beams
-    # behind 4,000 keys, 10 own ones -27 / -26 / -27, 300 -5 / -14 / -21, 600 +22 / 0 / -13; 4 x 16 behind 16,000, 10 own -158 / -158 / -144, 1,000
-    # -107 / -146 / -152)
-    OWN_KEYS = 200
-
-    def __init__(self, runner: "ModelRunner", bucket: int, beams: int = 0):
+    def __init__(self, runner: "ModelRunner", bucket: int, beams: int = 0, own: int = 0):
         self.bucket = bucket
         self.beams = beams
         P = runner.max_pages_per_request
@@ -167,7 +162,7 @@ class _DecodeGraph:
             num_tokens=bucket, num_entries=bucket, token_ids=v[0], positions=v[1], cu_q=v[2], kv_len=v[3],
             state_slots=v[4], groups=gsteps, entries=[], max_q_len=1,
             max_kv_len=runner.max_model_len, decode_only=True, indices=indices,
-            beams=beams, shared_len=v[-1] if beams > 1 else None, max_own_len=min(self.OWN_KEYS, runner.max_model_len) if beams > 1 else 0)
+            beams=beams, shared_len=v[-1] if beams > 1 else None, max_own_len=min(own, runner.max_model_len) if beams > 1 else 0)
         self.rows = v[5]
         # one eager run (libraries pick their algorithms, lazy kernels get built), then capture
         torch.cuda.synchronize()
@@ -202,9 +197,10 @@ class _DecodeGraph:
         """Every row's block table is written afresh at its next use."""
         self.row_owner = [-1] * self.bucket
 
-    def fill(self, runner: "ModelRunner", entries: Sequence[StepEntry], host_tokens: bool) -> None:
+    def fill(self, runner: "ModelRunner", entries: Sequence[StepEntry], host_tokens: bool, common: Sequence[int] = ()) -> None:
         """Write this step's indices into the pinned buffer and send it.  A row keeps the
-        block table of the request it held last step; only pages added since are written."""
+        block table of the request it held last step; only pages added since are written.
+        `common`: of a step of beams, the keys that each request's beams share."""
         if self.event is not None:
             self.event.synchronize()                         # the last upload has left the host buffer
         ps = runner.page_size
@@ -241,7 +237,6 @@ class _DecodeGraph:
                     raise StepError("a token would be written to a page that was given back")
                 self.h_slot_of_token[gi][i] = page * ps + pos % ps
         if self.h_shared is not None:
-            common = runner._common(entries, self.beams)
             self.h_shared[: len(common)] = common
             self.h_shared[len(common):] = 0
         for i in range(len(entries), self.bucket):           # padding rows
@@ -274,6 +269,11 @@ class ModelRunner:
     # Steps of beams read their requests' common keys together where that takes no longer (`attention_beams_sooner`); with a number here, where all
     # beams together see at least so many of them.  (Keys that a window hides are counted: no model with windows takes the kernel.)
     beam_keys: Optional[int] = None
+
+    # own keys a beam that captured steps of beams are cut for, the former while no beam has more than half as many again.  (us a layer against row by
+    # row, for cuts of 64 / 200 / 400, heads of 64: 8 x 8 beams behind 4,000 keys, 300 own ones -5 / -14 / -21, 600 +22 / 0 / -13; 4 x 16 behind
+    # 16,000, 10 own -158 / -158 / -144, 1,000 -107 / -146 / -152; with room for 4,200 keys a request, 8 x 8 and 20 own, 64 is 5 sooner than 200)
+    OWN_KEYS = (64, 200)
 
     def __init__(self, model_dir: str, dtype="bfloat16", device="cuda:0", max_model_len: int = 4096,
                  page_size: int = 16, num_pages: Optional[int] = None, max_batch_seqs: int = 64,
@@ -333,7 +333,7 @@ class ModelRunner:
         # (heads, key heads, head size) of the largest mixer that can read beams together
         self._beam_sizes = max(((m.Hq, m.Hkv, m.hd) for m in (b.mixer for b in self.model.blocks) if getattr(m, "use_mma", False)),
                                key=lambda s: s[1] * s[2], default=None)
-        self._graphs: Dict[Any, "_DecodeGraph"] = {}          # by rows; by (rows, beams a request) of steps of beams
+        self._graphs: Dict[Any, "_DecodeGraph"] = {}          # by rows; of steps of beams by (rows, beams a request), and their cut for own keys above the least
         self._graph_pool = None
         self.use_graphs = bool(self.capture_sizes) and self.model.graph_safe
 
@@ -478,18 +478,20 @@ class ModelRunner:
         """Keys that the requests of every `beams` entries have in common, as far as they were when they were forked."""
         return [self.cache.common_length([e.request_id for e in entries[i: i + beams]]) for i in range(0, len(entries), beams)]
 
-    def _together(self, entries: Sequence[StepEntry], beams: int) -> bool:
-        """Whether a step of beams reads its requests' common keys once for all of a request's beams, or row by row."""
-        if beams > _k.BEAMS_MAX:
-            return False
+    def _own(self, entries: Sequence[StepEntry], beams: int, common: Sequence[int]) -> int:
+        """Keys that the longest beam has behind the common ones, this step's among them."""
+        return max(self.cache.length(e.request_id) + 1 - c for e, c in zip(entries[::beams], common))
+
+    def _together(self, entries: Sequence[StepEntry], beams: int) -> List[int]:
+        """The keys that the requests of a step of beams have in common, if these are to be read once for all of a request's beams; else nothing."""
+        if beams > _k.BEAMS_MAX or (self.beam_keys is None and not self._beam_sizes):
+            return []
         common = self._common(entries, beams)
         keys = beams * sum(common)
         if self.beam_keys is not None:
-            return keys >= self.beam_keys
-        if not self._beam_sizes:
-            return False
-        own = max(self.cache.length(e.request_id) + 1 - c for e, c in zip(entries[::beams], common))
-        return _k.attention_beams_sooner(len(entries), beams, *self._beam_sizes, keys, own)
+            return common if keys >= self.beam_keys else []
+        sooner = _k.attention_beams_sooner(len(entries), beams, *self._beam_sizes, keys, self._own(entries, beams, common))
+        return common if sooner else []
 
     def _validate(self, entries: Sequence[StepEntry]) -> Optional[np.ndarray]:
         """Raises `StepError` for a step that cannot be; returns the ids of a step of many tokens as one array (None: as they are)."""
@@ -525,7 +527,8 @@ class ModelRunner:
             raise StepError(f"{total} tokens exceed max_batch_tokens {self.max_batch_tokens}")
         return ids
 
-    def _build(self, entries: Sequence[StepEntry], ids: Optional[np.ndarray], beams: int = 0) -> Tuple[StepContext, Optional[torch.Tensor]]:
+    def _build(self, entries: Sequence[StepEntry], ids: Optional[np.ndarray], beams: int = 0,
+               common: Sequence[int] = ()) -> Tuple[StepContext, Optional[torch.Tensor]]:
         ps = self.page_size
         B = len(entries)
         q_lens = np.fromiter((len(e.tokens) for e in entries), dtype=np.int64, count=B)
@@ -566,7 +569,7 @@ class ModelRunner:
         sections.append(np.asarray(row_slots, dtype=np.int64))
         shared = None
         if beams > 1:
-            shared = np.asarray(self._common(entries, beams), dtype=np.int64)
+            shared = np.asarray(common, dtype=np.int64)
             sections.append(shared)
         shape = StepShape(q_lens, pos0, cu_q, kv_len, slots)
         built = [(need, need.build(shape)) for need in self.index_needs]
@@ -621,18 +624,19 @@ class ModelRunner:
         ids = self._validate(entries)
         if beams > 1 and (len(entries) % beams or any(len(e.tokens) != 1 for e in entries)):
             raise StepError(f"{len(entries)} entries are no single tokens of {beams} beams a request")
-        if beams > 1 and not self._together(entries, beams):
+        common = self._together(entries, beams) if beams > 1 else []
+        if not common:
             beams = 0
         lease = self.cache.lease([(e.request_id, len(e.tokens)) for e in entries])
         try:
             self._zero_new_state()
             bucket, beams = self._bucket_for(entries, beams)
             if bucket:
-                logits = self._graph_step(entries, bucket, device_tokens, beams)
+                logits = self._graph_step(entries, bucket, device_tokens, beams, common)
                 if logits is not None and not borrow_logits:
                     logits = logits.clone()
             else:
-                step, rows = self._build(entries, ids, beams)
+                step, rows = self._build(entries, ids, beams, common)
                 if device_tokens is not None:
                     if not step.decode_only:
                         raise StepError("device_tokens only stands for steps of single tokens")
@@ -665,13 +669,17 @@ class ModelRunner:
         return 0, beams
 
     def _graph_step(self, entries: Sequence[StepEntry], bucket: int,
-                    device_tokens: Optional[torch.Tensor], beams: int = 0) -> Optional[torch.Tensor]:
-        key = (bucket, beams) if beams > 1 else bucket
+                    device_tokens: Optional[torch.Tensor], beams: int = 0, common: Sequence[int] = ()) -> Optional[torch.Tensor]:
+        key, own = bucket, 0
+        if beams > 1:
+            few, many = self.OWN_KEYS
+            own = few if 2 * self._own(entries, beams, common) <= 3 * few else many
+            key = (bucket, beams) if own == few else (bucket, beams, own)
         g = self._graphs.get(key)
         if g is None:
-            g = _DecodeGraph(self, bucket, beams)
+            g = _DecodeGraph(self, bucket, beams, own)
             self._graphs[key] = g
-        g.fill(self, entries, device_tokens is None)
+        g.fill(self, entries, device_tokens is None, common)
         if device_tokens is not None:
             g.step.token_ids[: len(entries)].copy_(device_tokens[: len(entries)])
         g.graph.replay()

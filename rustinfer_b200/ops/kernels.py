@@ -2187,8 +2187,8 @@ def _attention_beams_plan(rows: int, beams: int, num_heads: int, num_kv_heads: i
     enough of it for the rows' own keys: by about 6 us and 2 a tile of 64 keys for the former, 3 us and 1 a step of 16 for a row's warp, both
     for heads of 64.  (Over 23 shapes 3 % behind the best cut of each, 9 % at most.  us, against a fixed 6 or 7 eighths with ranges of 32 own
     keys: 4 x 16 beams, heads of 128, of 9,001 and 100 keys 44 and 53, of 2,000 and 300 31 and 36, of 9,001 and 1,000 71 and 84; 8 x 8,
-    heads of 64, of 4,096 and 1,000 52 and 62.  These are calls that say how many own keys there are, as eager steps do; a captured step says 200
-    for as long as it lives.)"""
+    heads of 64, of 4,096 and 1,000 52 and 62.  These are calls that say how many own keys there are, as eager steps do; captured steps say 64
+    or 200.)"""
     if not attention_beams_supports(num_heads, num_kv_heads, head_dim):
         raise KernelError(f"attention_decode_beams: {num_heads} heads over {num_kv_heads} of {head_dim} (a multiple of 16 up to {L.MMA_MAX_HEAD_DIM})")
     if not 1 <= beams <= BEAMS_MAX or rows % beams:

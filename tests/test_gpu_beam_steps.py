@@ -186,3 +186,28 @@ def test_steps_take_the_sooner_way(tmp_path):
             r._graphs.clear()
             x = r.step([StepEntry(i, [5], [0]) for i in ids], beams=4)
             assert bool(x.isfinite().all()) and list(r._graphs) == [(8, 4) if chosen else 8], (dtype, families, common, own)
+
+
+@pytest.mark.parametrize("name", ["A", "D", "E"])
+def test_captured_steps_by_their_own_keys(folder, calls, name):
+    """Beams with more than 96 keys of their own run from a captured step that is cut for more; both read what they should."""
+    from rustinfer_b200.engine.runner import StepEntry
+    r = _runner(folder(name), max_model_len=512, num_pages=150, capture_sizes=[6])
+    vocab, held, order = r.spec.vocab_size, Held(r), [f + k for f in "ab" for k in "012"]
+    saved, common = {}, [50, 96]
+    for f, n in zip("ab", common):
+        r.open(f + "0")
+        r.step([StepEntry(f + "0", random_ids(n, vocab, n), [0])])
+        r.fork(f + "0", [f + "1", f + "2"])
+        held.add(f + "0", n)
+        held.kv.update({f + k: held.kv[f + "0"] for k in "12"})
+    for at, (own, key) in enumerate(((0, (6, 3)), (95, (6, 3)), (96, (6, 3, 200)), (230, (6, 3, 200)))):
+        for i in order:
+            more = own + common["ab".index(i[0])] - r.cache.length(i)
+            if more > 0:
+                r.step([StepEntry(i, random_ids(more, vocab, 7 * at + order.index(i)), [])])
+                held.add(i, r.cache.length(i))
+        _step_and_check(r, held, calls, saved.setdefault(key, []), order, 3, 50 + at, common)
+        assert key in r._graphs and len(r._graphs) == 1 + (own >= 96)
+        r.reorder(order, [1, 1, 0, 3, 5, 4], 3)
+        held.kv = {i: held.kv[order[p]] for i, p in zip(order, [1, 1, 0, 3, 5, 4])}
