@@ -15,7 +15,7 @@ MEASURED = [
     (32, 8, 128, 16, 4, 1000, 1000, 249, 256), (32, 8, 128, 12, 4, 1378, 400, 258, 219), (32, 8, 128, 1, 4, 16547, 60, 192, 190),
     (32, 8, 128, 1, 4, 16000, 1000, 192, 231), (32, 8, 128, 1, 64, 4000, 600, 315, 239), (32, 8, 128, 16, 2, 1536, 150, 173, 183),
     (32, 8, 128, 16, 2, 4116, 400, 216, 229), (32, 8, 128, 1, 16, 8232, 250, 353, 320), (24, 8, 128, 1, 8, 8273, 60, 135, 127),
-    (24, 8, 128, 4, 4, 4136, 400, 164, 168), (24, 8, 128, 1, 16, 3072, 400, 156, 162), (32, 8, 128, 2, 2, 32931, 10, 219, 213),
+    (24, 8, 128, 4, 4, 4136, 400, 164, 168), (32, 8, 128, 2, 2, 32931, 10, 219, 213),
     (32, 8, 128, 1, 4, 300, 10, 164, 168), (24, 8, 128, 8, 8, 1536, 400, 193, 168)]
 
 
